@@ -71,7 +71,8 @@ int nb200_attn_fwd(const void *q, const void *k, const void *v, void *out,
                    float scale_log2, int causal, int *status, void *stream);
 
 /* Copies a status buffer to the host after synchronising `stream`; returns NB200_OK if status[0] is clear,
- * NB200_ERR_BAD_ARG if a kernel refused device-side data (code 22: a block-table entry outside the page pool),
+ * NB200_ERR_BAD_ARG if a kernel refused device-side data (code 22: a block-table entry outside the page pool;
+ * code 23: an appended row whose position its block-table row does not reach),
  * NB200_ERR_DEVICE_TIMEOUT for every other code (an expired bounded wait). host_out may be NULL.
  * A non-zero status[0] makes later attention and SSD launches that are given the same buffer return at once
  * without touching their outputs, so read it (and zero it) after synchronising whenever a result matters. */
@@ -244,6 +245,76 @@ int nb200_peer_buffer_free(void *ptr);
 int nb200_decode_fwd_static(const void *q, const void *k, const void *v, void *out,
                             int B, int Hq, int Hkv, int Lkv, int D, int n_splits, int dtype,
                             float scale_log2, void *stream);
+
+/*
+ * Norm of every query and key head with the position rotation in the same pass (no counterpart in the reference):
+ * what a layer does between its projection and nb200_attn_fwd.  For a row x of D elements at position p
+ *
+ *   y = x * rsqrt(mean(x^2) + eps) * weight                        (weight NULL: no norm, y = x)
+ *   (y1, y2) <- (y1 cos a - y2 sin a, y2 cos a + y1 sin a),        a = p * inv_freq[i], i < rot_dim / 2
+ *
+ * over the pairs (i, i + rot_dim / 2), or (2i, 2i + 1) if `interleaved`; elements from rot_dim on are not rotated.
+ * Computed in fp32 (the angle's reduction in fp64, so that positions of many thousand turns stay exact) and rounded once.
+ *
+ *   q [B, S, Hq, D]   k [B, S, Hkv, D]   q_out, k_out the same   (f16, bf16 or f32; D a multiple of 16, D <= 256)
+ *   q_weight, k_weight : [D] in the tensors' dtype, or NULL
+ *   inv_freq  : fp32 [rot_dim / 2], rot_dim a multiple of 16, 16 <= rot_dim <= D
+ *   positions : int32 [B, S] (any value, negative ones too)
+ *   strides   : HOST array of 13: the batch, token and head stride (in elements) of q, k, q_out and k_out in this order,
+ *               then the batch stride of positions (0: one row for all).  Rows are contiguous; strides and base
+ *               addresses are multiples of 16 bytes.  So q and k may be views into a packed projection and q_out,
+ *               k_out [B, H, S, D] tensors as nb200_attn_fwd reads them.
+ * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.
+ */
+int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, const int *positions,
+                       const float *inv_freq, const void *q_weight, const void *k_weight, const long long *strides,
+                       int B, int S, int Hq, int Hkv, int D, int rot_dim, int interleaved, float eps, int dtype,
+                       void *stream);
+
+/*
+ * Append of new tokens to the paged KV cache of nb200_decode_paged_splitk, with the norms and the rotation of
+ * nb200_qk_norm_rope on the way (no counterpart in the reference).  The batch is ragged: rows
+ * cu_seqlens[b] .. cu_seqlens[b+1]-1 are the LAST tokens of sequence b, whose length with them is seq_lens[b]; row t is
+ * at position p = seq_lens[b] - cu_seqlens[b+1] + t, and its key (normed, rotated by p) and value (as it is) go to row
+ * p % 64 of page block_table[b, p / 64].  One token per sequence is a decode step.
+ *
+ *   q [T, Hq, D]   k, v [T, Hkv, D]   q_out [T, Hq, D]     (f16 or bf16, D == 128; q may be absent: Hq = 0)
+ *   k_pages, v_pages, block_table, num_pages, max_pages, page_size : as for nb200_decode_paged_splitk
+ *   cu_seqlens : int32 [B + 1], not decreasing      seq_lens : int32 [B]
+ *   q_weight, k_weight, inv_freq, rot_dim, interleaved, eps : as for nb200_qk_norm_rope
+ *   strides    : HOST array of 8: the token and head stride (in elements) of q, k, v and q_out; rules as above
+ * Rows that belong to no sequence (before cu_seqlens[0], from cu_seqlens[B] on) are not touched, in q_out as in the
+ * cache.  Of a row whose position is outside its row of the block table, or whose page is outside the pool, nothing
+ * is written and `status` (may be NULL) records code 23 with the row and the position, or code 22 with the entry, which
+ * nb200_status_read reports as NB200_ERR_BAD_ARG.  Two sequences of one call must not append to the same page.
+ * q_out may be q (same address and strides); otherwise outputs share no element with inputs.
+ */
+int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, void *k_pages, void *v_pages,
+                      const int *block_table, const int *cu_seqlens, const int *seq_lens, const float *inv_freq,
+                      const void *q_weight, const void *k_weight, const long long *strides, int T, int B, int Hq,
+                      int Hkv, int num_pages, int max_pages, int page_size, int D, int rot_dim, int interleaved,
+                      float eps, int dtype, int *status, void *stream);
+
+/*
+ * Attention of the new tokens of such a ragged batch over the paged cache that already holds them (no counterpart in
+ * the reference): prompt chunks, drafted tokens and single decode tokens in one call.  Row t of sequence b, at position
+ * p as above, sees the cached rows j <= p (at most max_pages * 64 of them).
+ *
+ *   q, out [T, Hq, D]   (f16 or bf16, D == 128, Hq % Hkv == 0)   pools, table, cu_seqlens, seq_lens as above
+ *   workspace  : nb200_attn_paged_workspace_bytes() bytes, 16-byte aligned, need not be cleared.  Calls that can overlap
+ *                on the GPU need one each.
+ *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out; not negative, rules as above
+ *   scale_log2 : log2(e) * softmax scale
+ * A row that sees nothing (its position is negative) is 0; rows that belong to no sequence are not touched.  Cache rows
+ * at and beyond a sequence's length are not used, whatever they hold.  A table entry outside [0, num_pages) is never
+ * dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and
+ * `status` records code 22.
+ */
+size_t nb200_attn_paged_workspace_bytes(void);
+int nb200_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int *block_table,
+                     const int *cu_seqlens, const int *seq_lens, void *workspace, void *out, const long long *strides,
+                     int T, int B, int Hq, int Hkv, int num_pages, int max_pages, int page_size, int D, int dtype,
+                     float scale_log2, int *status, void *stream);
 
 /*
  * Mamba-1 selective scan forward (no counterpart in the reference).

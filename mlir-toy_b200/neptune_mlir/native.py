@@ -47,6 +47,10 @@ SYMBOLS: dict[str, tuple] = {
     "nb200_peer_buffer_free": (c_int, [c_void_p]),
     "nb200_decode_fwd_static": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                         c_int, c_int, c_float, c_void_p]),
+    "nb200_qk_norm_rope": (c_int, [c_void_p] * 9 + [c_int] * 7 + [c_float, c_int, c_void_p]),
+    "nb200_rope_append": (c_int, [c_void_p] * 13 + [c_int] * 10 + [c_float, c_int, c_void_p, c_void_p]),
+    "nb200_attn_paged_workspace_bytes": (c_size_t, []),
+    "nb200_attn_paged": (c_int, [c_void_p] * 9 + [c_int] * 9 + [c_float, c_void_p, c_void_p]),
     "nb200_selective_scan_fwd": (c_int, [c_void_p] * 8 + [c_int] * 5 + [c_void_p]),
     "nb200_ssd_workspace_bytes": (c_size_t, [c_int] * 7),
     "nb200_ssd_launches": (c_int, [c_int] * 7),

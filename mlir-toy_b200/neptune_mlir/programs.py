@@ -372,6 +372,45 @@ def decode_paged_decl(name: str, B: int, Hq: int, Hkv: int, num_pages: int, max_
     ], {"htile.operator": "decode_paged", "n_splits": n_splits, "scale": _f32(1.0 / math.sqrt(D))})
 
 
+def qk_norm_rope_decl(name: str, B: int, S: int, Hq: int, Hkv: int, D: int, rot_dim: int, norm: bool = True,
+                      interleaved: bool = False, eps: float = 1e-6, dtype: str = "bf16") -> str:
+    """Declaration of per-head norm and rotation: (q, k, positions, inv_freq, q_out, k_out[, q_weight, k_weight])."""
+    args = [("q", f"memref<{B}x{S}x{Hq}x{D}x{dtype}>"), ("k", f"memref<{B}x{S}x{Hkv}x{D}x{dtype}>"),
+            ("positions", f"memref<{B}x{S}xi32>"), ("inv_freq", f"memref<{rot_dim // 2}xf32>"),
+            ("q_out", f"memref<{B}x{Hq}x{S}x{D}x{dtype}>"), ("k_out", f"memref<{B}x{Hkv}x{S}x{D}x{dtype}>")]
+    if norm:
+        args += [("q_weight", f"memref<{D}x{dtype}>"), ("k_weight", f"memref<{D}x{dtype}>")]
+    return _decl(name, args, {"htile.operator": "qk_norm_rope", "interleaved": int(interleaved), "eps": _f32(eps)})
+
+
+def rope_append_decl(name: str, T: int, B: int, Hq: int, Hkv: int, num_pages: int, max_pages: int, D: int, rot_dim: int,
+                     norm: bool = True, interleaved: bool = False, eps: float = 1e-6, page_size: int = 64,
+                     dtype: str = "bf16") -> str:
+    """Declaration of the append to a paged KV cache: (q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens,
+    inv_freq, q_out[, q_weight, k_weight])."""
+    pool = f"memref<{num_pages}x{Hkv}x{page_size}x{D}x{dtype}>"
+    q, kv = f"memref<{T}x{Hq}x{D}x{dtype}>", f"memref<{T}x{Hkv}x{D}x{dtype}>"
+    args = [("q", q), ("k", kv), ("v", kv), ("k_pages", pool), ("v_pages", pool),
+            ("block_table", f"memref<{B}x{max_pages}xi32>"), ("cu_seqlens", f"memref<{B + 1}xi32>"),
+            ("seq_lens", f"memref<{B}xi32>"), ("inv_freq", f"memref<{rot_dim // 2}xf32>"), ("q_out", q)]
+    if norm:
+        args += [("q_weight", f"memref<{D}x{dtype}>"), ("k_weight", f"memref<{D}x{dtype}>")]
+    return _decl(name, args, {"htile.operator": "rope_append", "interleaved": int(interleaved), "eps": _f32(eps)})
+
+
+def attn_paged_decl(name: str, T: int, B: int, Hq: int, Hkv: int, num_pages: int, max_pages: int, D: int,
+                    workspace_bytes: int, page_size: int = 64, dtype: str = "bf16") -> str:
+    """Declaration of the attention of new tokens over a paged KV cache: (q, k_pages, v_pages, block_table, cu_seqlens,
+    seq_lens, workspace, out)."""
+    pool = f"memref<{num_pages}x{Hkv}x{page_size}x{D}x{dtype}>"
+    q = f"memref<{T}x{Hq}x{D}x{dtype}>"
+    return _decl(name, [
+        ("q", q), ("k_pages", pool), ("v_pages", pool), ("block_table", f"memref<{B}x{max_pages}xi32>"),
+        ("cu_seqlens", f"memref<{B + 1}xi32>"), ("seq_lens", f"memref<{B}xi32>"),
+        ("workspace", f"memref<{workspace_bytes}xi8>"), ("out", q),
+    ], {"htile.operator": "attn_paged", "scale": _f32(1.0 / math.sqrt(D))})
+
+
 def selective_scan_decl(name: str, B: int, Dm: int, L: int, N: int = 16, dtype: str = "bf16") -> str:
     """Declaration of the Mamba-1 selective scan: (u, delta, A, B, C, D, z, out)."""
     seq = f"memref<{B}x{Dm}x{L}x{dtype}>"

@@ -11,6 +11,8 @@ the kernel library every call raises.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import native
@@ -43,6 +45,45 @@ def _same_device(*tensors) -> torch.device:
 
 def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _rows(name: str, t, shape, dtype: str) -> tuple:
+    """Check a tensor whose rows (last dimension) are contiguous and whose other strides are free; return those."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor (the B200 target has no CPU path)")
+    if t.dtype != _TORCH_DTYPES[dtype]:
+        raise TypeError(f"{name}: dtype {t.dtype}, the program says {_TORCH_DTYPES[dtype]}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, the program says {tuple(shape)}")
+    strides = t.stride()
+    if strides[-1] != 1:
+        raise ValueError(f"{name}: rows must be contiguous")
+    return strides[:-1]
+
+
+def _pools(k_pages, v_pages, Hkv: int, page_size: int, D: int, dtype: str) -> int:
+    """Check the two page pools of a paged cache; return their number of pages."""
+    want = _TORCH_DTYPES[dtype]
+    for name, pool in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if not (isinstance(pool, torch.Tensor) and pool.is_cuda and pool.is_contiguous() and pool.dim() == 4
+                and pool.shape[1:] == (Hkv, page_size, D) and pool.dtype == want):
+            raise ValueError(f"{name}: expected a contiguous CUDA [num_pages, {Hkv}, {page_size}, {D}] {dtype} tensor")
+    if k_pages.shape[0] != v_pages.shape[0]:
+        raise ValueError("k_pages and v_pages must hold the same number of pages")
+    return k_pages.shape[0]
+
+
+def _launch(fn, what: str, dev: torch.device, *args) -> None:
+    """Call a C entry point with ``dev`` current and its current stream as the last argument."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(dev))
+    if rc:
+        native.check(rc, what)
 
 
 def status_buffer(dev: torch.device) -> torch.Tensor:
@@ -173,6 +214,105 @@ def decode_merge_nccl(local_partial, gathered, out, *, rows, D, world, out_dtype
                                                   rows, D, world, native.DTYPE_CODES[out_dtype], comm.handle,
                                                   _stream(dev))
     native.check(rc, "nb200_decode_merge_nccl")
+
+
+def _norm_weight(name: str, w, D: int, dtype: str):
+    if w is None:
+        return None
+    _check(name, w, (D,), dtype)
+    return w.data_ptr()
+
+
+def _one_device(*tensors) -> torch.device:
+    """The device of all the tensors that are not None."""
+    return _same_device(*[t for t in tensors if t is not None])
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_out, k_out, q_weight=None, k_weight=None, *, B, S, Hq, Hkv, D, rot_dim,
+                 interleaved, eps, dtype) -> None:
+    """Norm of every query and key head (where it has weights) and position rotation, in one pass.
+
+    q [B, S, Hq, D] and k [B, S, Hkv, D] are token-major, as a projection leaves them; q_out [B, Hq, S, D] and
+    k_out [B, Hkv, S, D] head-major, as ``attn_fwd`` reads them.  Rows of D are contiguous, the other strides free
+    multiples of 16 bytes (so an output may also be its input's ``transpose(1, 2)``, in place).  positions is int32
+    [S] or [B, S], inv_freq fp32 [rot_dim / 2]; the weights are [D].
+    """
+    qs = _rows("q", q, (B, S, Hq, D), dtype)
+    ks = _rows("k", k, (B, S, Hkv, D), dtype)
+    qo = _rows("q_out", q_out, (B, Hq, S, D), dtype)
+    ko = _rows("k_out", k_out, (B, Hkv, S, D), dtype)
+    one_row = isinstance(positions, torch.Tensor) and positions.dim() == 1
+    _check("positions", positions, (S,) if one_row else (B, S), torch.int32)
+    _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
+    wq, wk = _norm_weight("q_weight", q_weight, D, dtype), _norm_weight("k_weight", k_weight, D, dtype)
+    dev = _one_device(q, k, positions, inv_freq, q_out, k_out, q_weight, k_weight)
+    strides = (ctypes.c_longlong * 13)(*qs, *ks, qo[0], qo[2], qo[1], ko[0], ko[2], ko[1], 0 if one_row else S)
+    _launch(native.lib().nb200_qk_norm_rope, "nb200_qk_norm_rope", dev, q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
+            k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), wq, wk, strides, B, S, Hq, Hkv, D, rot_dim,
+            int(bool(interleaved)), eps, native.DTYPE_CODES[dtype])
+
+
+def rope_append(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, q_out, q_weight=None,
+                k_weight=None, *, T, B, Hq, Hkv, max_pages, page_size, D, rot_dim, interleaved, eps, dtype) -> None:
+    """Append a ragged batch of new tokens to the paged cache of ``decode_paged``, normed and rotated on the way.
+
+    Rows cu_seqlens[b] .. cu_seqlens[b+1]-1 of k, v [T, Hkv, D] are the last tokens of sequence b, seq_lens[b] its
+    length with them; q [T, Hq, D] is rotated into q_out the same way (both None with Hq = 0: keys and values only).
+    Rows of D are contiguous, the other strides free multiples of 16 bytes; q_out may be q.  Positions or pages that
+    the table or the pool does not have are reported by ``check_status``.
+    """
+    if Hq == 0:
+        if q is not None or q_out is not None:
+            raise ValueError("rope_append: Hq = 0 goes with q = q_out = None")
+        qs = qo = (0, 0)
+    else:
+        qs = _rows("q", q, (T, Hq, D), dtype)
+        qo = _rows("q_out", q_out, (T, Hq, D), dtype)
+    ks = _rows("k", k, (T, Hkv, D), dtype)
+    vs = _rows("v", v, (T, Hkv, D), dtype)
+    pages = _pools(k_pages, v_pages, Hkv, page_size, D, dtype)
+    _check("block_table", block_table, (B, max_pages), torch.int32)
+    _check("cu_seqlens", cu_seqlens, (B + 1,), torch.int32)
+    _check("seq_lens", seq_lens, (B,), torch.int32)
+    _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
+    wq, wk = _norm_weight("q_weight", q_weight, D, dtype), _norm_weight("k_weight", k_weight, D, dtype)
+    dev = _one_device(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, q_out, q_weight, k_weight)
+    strides = (ctypes.c_longlong * 8)(*qs, *ks, *vs, *qo)
+    _launch(native.lib().nb200_rope_append, "nb200_rope_append", dev, q.data_ptr() if Hq else None, k.data_ptr(),
+            v.data_ptr(), q_out.data_ptr() if Hq else None, k_pages.data_ptr(), v_pages.data_ptr(),
+            block_table.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), inv_freq.data_ptr(), wq, wk, strides, T,
+            B, Hq, Hkv, pages, max_pages, page_size, D, rot_dim, int(bool(interleaved)), eps,
+            native.DTYPE_CODES[dtype], status_buffer(dev).data_ptr())
+
+
+def attn_paged_workspace_bytes() -> int:
+    """Scratch memory of one ``attn_paged`` call, whatever its sizes."""
+    return native.lib().nb200_attn_paged_workspace_bytes()
+
+
+def attn_paged(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out, *, T, B, Hq, Hkv, max_pages,
+               page_size, D, dtype, scale_log2) -> None:
+    """Attention of a ragged batch of new tokens (see ``rope_append``) over the paged cache that holds them already.
+
+    q, out [T, Hq, D] with contiguous rows and token and head strides that are multiples of 16 bytes; workspace is a
+    uint8 tensor of attn_paged_workspace_bytes(), one for each call that can run at the same time.
+    """
+    qs = _rows("q", q, (T, Hq, D), dtype)
+    outs = _rows("out", out, (T, Hq, D), dtype)
+    pages = _pools(k_pages, v_pages, Hkv, page_size, D, dtype)
+    _check("block_table", block_table, (B, max_pages), torch.int32)
+    _check("cu_seqlens", cu_seqlens, (B + 1,), torch.int32)
+    _check("seq_lens", seq_lens, (B,), torch.int32)
+    need = attn_paged_workspace_bytes()
+    if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
+            and workspace.numel() * workspace.element_size() >= need):
+        raise ValueError(f"workspace: need a contiguous CUDA tensor of at least {need} bytes")
+    dev = _same_device(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out)
+    strides = (ctypes.c_longlong * 4)(*qs, *outs)
+    _launch(native.lib().nb200_attn_paged, "nb200_attn_paged", dev, q.data_ptr(), k_pages.data_ptr(),
+            v_pages.data_ptr(), block_table.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(),
+            workspace.data_ptr(), out.data_ptr(), strides, T, B, Hq, Hkv, pages, max_pages, page_size, D,
+            native.DTYPE_CODES[dtype], scale_log2, status_buffer(dev).data_ptr())
 
 
 def selective_scan(u, delta, A, Bm, Cm, Dskip, z, out, *, B, Dm, L, N, dtype) -> None:

@@ -11,6 +11,7 @@ registers the ops; nothing else in the package depends on it.
 from __future__ import annotations
 
 import math
+from typing import Optional
 
 import torch
 
@@ -53,6 +54,40 @@ def decode_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
                          dtype=_name(q), scale_log2=math.log2(math.e) * scale)
 
 
+@torch.library.custom_op("nb200::qk_norm_rope", mutates_args=("q_out", "k_out"))
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_out: torch.Tensor,
+                 k_out: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor], eps: float,
+                 interleaved: bool) -> None:
+    """Per-head norm and rotation: q [B, S, Hq, D], k [B, S, Hkv, D], outputs [B, H, S, D], inv_freq fp32 [rot_dim / 2]."""
+    B, S, Hq, D = q.shape
+    runtime.qk_norm_rope(q, k, positions, inv_freq, q_out, k_out, q_weight, k_weight, B=B, S=S, Hq=Hq, Hkv=k.shape[2],
+                         D=D, rot_dim=2 * inv_freq.shape[0], interleaved=interleaved, eps=eps, dtype=_name(q))
+
+
+@torch.library.custom_op("nb200::rope_append", mutates_args=("k_pages", "v_pages", "q_out"))
+def rope_append(q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                block_table: torch.Tensor, cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, inv_freq: torch.Tensor,
+                q_out: Optional[torch.Tensor], q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                eps: float, interleaved: bool) -> None:
+    """Append k, v [T, Hkv, D] of a ragged batch to the paged cache, normed and rotated; q [T, Hq, D] into q_out."""
+    T, Hkv, D = k.shape
+    runtime.rope_append(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, q_out, q_weight,
+                        k_weight, T=T, B=block_table.shape[0], Hq=0 if q is None else q.shape[1], Hkv=Hkv,
+                        max_pages=block_table.shape[1], page_size=k_pages.shape[2], D=D, rot_dim=2 * inv_freq.shape[0],
+                        interleaved=interleaved, eps=eps, dtype=_name(k))
+
+
+@torch.library.custom_op("nb200::attn_paged", mutates_args=("workspace", "out"))
+def attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+               cu_seqlens: torch.Tensor, seq_lens: torch.Tensor, workspace: torch.Tensor, out: torch.Tensor,
+               scale: float) -> None:
+    """Attention of a ragged batch of new tokens q [T, Hq, D] over the paged cache; workspace uint8."""
+    T, Hq, D = q.shape
+    runtime.attn_paged(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out, T=T,
+                       B=block_table.shape[0], Hq=Hq, Hkv=k_pages.shape[1], max_pages=block_table.shape[1],
+                       page_size=k_pages.shape[2], D=D, dtype=_name(q), scale_log2=math.log2(math.e) * scale)
+
+
 @torch.library.custom_op("nb200::selective_scan", mutates_args=("out",))
 def selective_scan(u: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor,
                    Dskip: torch.Tensor, z: torch.Tensor, out: torch.Tensor) -> None:
@@ -70,4 +105,4 @@ def ssd_chunk_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch
                            chunk=chunk, dtype=_name(x))
 
 
-OPS = ("attn_fwd", "decode_splitk", "decode_paged", "selective_scan", "ssd_chunk_scan")
+OPS = ("attn_fwd", "decode_splitk", "decode_paged", "qk_norm_rope", "rope_append", "attn_paged", "selective_scan", "ssd_chunk_scan")

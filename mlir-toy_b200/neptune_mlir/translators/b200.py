@@ -21,7 +21,8 @@ function onto one hand-written kernel family.  It therefore *recognises* program
   ``neptune_mlir.programs.decode_splitk_htile`` writes it): both regions are compared with the operator's
   equations and B, Hq, Hkv, L, D, the split count and the scale are read off them;
 * operator declarations: a ``func.func`` with attribute ``htile.operator`` naming one of
-  ``decode_splitk``, ``selective_scan``, ``ssd_chunk_scan`` and an empty body; the memref
+  ``decode_splitk``, ``decode_paged``, ``qk_norm_rope``, ``rope_append``, ``attn_paged``, ``selective_scan``,
+  ``ssd_chunk_scan`` and an empty body; the memref
   argument types carry the problem sizes.  The dialect has no scan op
   (include/HTile/HTileOps.td:21-217), so these operators cannot be spelled op by op.
 
@@ -231,6 +232,53 @@ class Translator:
             scale = float(fn.attributes.get("scale", 1.0 / math.sqrt(D)))
             return self._runtime_call("decode_paged", params, B=B, Hq=Hq, Hkv=Hkv, max_pages=table[1], page_size=page,
                                       D=D, n_splits=n_splits, dtype=dts[0], scale_log2=scale * math.log2(math.e))
+        if operator == "qk_norm_rope":
+            need(len(types) in (6, 8), "expects (q, k, positions, inv_freq, q_out, k_out[, q_weight, k_weight])")
+            q, k, pos, freq, qo, ko = shapes[:6]
+            need(len(q) == 4 and len(k) == 4 and k[:2] == q[:2] and k[3] == q[3], "q [B,S,Hq,D], k [B,S,Hkv,D]")
+            B, S, Hq, D = q
+            Hkv = k[2]
+            need(qo == (B, Hq, S, D) and ko == (B, Hkv, S, D), "q_out [B,Hq,S,D], k_out [B,Hkv,S,D]")
+            need(pos in ((S,), (B, S)) and dts[2] == "i32" and len(freq) == 1 and dts[3] == "f32",
+                 "positions memref<[Bx]Sxi32>, inv_freq memref<Rxf32>")
+            need(all(w == (D,) for w in shapes[6:]), "weights memref<D>")
+            need(dts[0] in ("f16", "bf16", "f32") and all(dts[i] == dts[0] for i in (1, *range(4, len(dts)))),
+                 "q/k/outputs/weights share f16, bf16 or f32")
+            return self._runtime_call("qk_norm_rope", params, B=B, S=S, Hq=Hq, Hkv=Hkv, D=D, rot_dim=2 * freq[0],
+                                      interleaved=bool(fn.attributes.get("interleaved", 0)),
+                                      eps=float(fn.attributes.get("eps", 1e-6)), dtype=dts[0])
+        if operator == "rope_append":
+            need(len(types) in (10, 12), "expects (q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, "
+                                         "q_out[, q_weight, k_weight])")
+            q, k, v, kp, vp, table, cu, lens, freq, qo = shapes[:10]
+            need(len(q) == 3 and qo == q and len(k) == 3 and k == v and k[0] == q[0] and k[2] == q[2],
+                 "q/q_out [T,Hq,D], k/v [T,Hkv,D]")
+            T, Hq, D = q
+            need(len(kp) == 4 and kp == vp and kp[1] == k[1] and kp[3] == D, "pools [pages,Hkv,page,D]")
+            need(len(table) == 2 and cu == (table[0] + 1,) and lens == (table[0],) and dts[5] == dts[6] == dts[7] == "i32",
+                 "block_table memref<Bxmax_pagesxi32>, cu_seqlens memref<(B+1)xi32>, seq_lens memref<Bxi32>")
+            need(len(freq) == 1 and dts[8] == "f32", "inv_freq memref<Rxf32>")
+            need(all(w == (D,) for w in shapes[10:]), "weights memref<D>")
+            need(dts[0] in ("f16", "bf16") and all(dts[i] == dts[0] for i in (1, 2, 3, 4, *range(9, len(dts)))),
+                 "q/k/v/pools/q_out/weights share f16 or bf16")
+            return self._runtime_call("rope_append", params, T=T, B=table[0], Hq=Hq, Hkv=k[1], max_pages=table[1],
+                                      page_size=kp[2], D=D, rot_dim=2 * freq[0],
+                                      interleaved=bool(fn.attributes.get("interleaved", 0)),
+                                      eps=float(fn.attributes.get("eps", 1e-6)), dtype=dts[0])
+        if operator == "attn_paged":
+            need(len(types) == 8, "expects (q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out)")
+            q, kp, vp, table, cu, lens, ws, out = shapes
+            need(len(q) == 3 and out == q and len(kp) == 4 and kp == vp, "q/out [T,Hq,D], pools [pages,Hkv,page,D]")
+            T, Hq, D = q
+            Hkv, page = kp[1], kp[2]
+            need(kp[3] == D and Hq % Hkv == 0, "inconsistent extents")
+            need(len(table) == 2 and cu == (table[0] + 1,) and lens == (table[0],) and dts[3] == dts[4] == dts[5] == "i32",
+                 "block_table memref<Bxmax_pagesxi32>, cu_seqlens memref<(B+1)xi32>, seq_lens memref<Bxi32>")
+            need(len(ws) == 1 and dts[6] == "i8", "workspace memref<Nxi8>")
+            need(dts[0] in ("f16", "bf16") and dts[0] == dts[1] == dts[2] == dts[7], "q/pools/out share f16 or bf16")
+            scale = float(fn.attributes.get("scale", 1.0 / math.sqrt(D)))
+            return self._runtime_call("attn_paged", params, T=T, B=table[0], Hq=Hq, Hkv=Hkv, max_pages=table[1],
+                                      page_size=page, D=D, dtype=dts[0], scale_log2=scale * math.log2(math.e))
         if operator == "selective_scan":
             need(len(types) == 8, "expects (u, delta, A, B, C, D, z, out)")
             u, dl, A, Bm, Cm, Dk, z, out = shapes
