@@ -303,7 +303,8 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  *   q, out [T, Hq, D]   (f16 or bf16, D == 128, Hq % Hkv == 0)   pools, table, cu_seqlens, seq_lens as above
  *   workspace  : nb200_attn_paged_workspace_bytes() bytes, 16-byte aligned, need not be cleared.  Calls that can overlap
  *                on the GPU need one each.
- *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out; not negative, rules as above
+ *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out: multiples of 16 bytes, at least a row (the
+ *                stride of an extent of 1 is not used)
  *   scale_log2 : log2(e) * softmax scale
  * A row that sees nothing (its position is negative) is 0; rows that belong to no sequence are not touched.  Cache rows
  * at and beyond a sequence's length are not used, whatever they hold.  A table entry outside [0, num_pages) is never

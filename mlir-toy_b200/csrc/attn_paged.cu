@@ -1,71 +1,839 @@
-// Attention of the new tokens of a ragged batch over the paged KV cache.
+// Attention of the new tokens of a ragged batch over the paged KV cache (f16 / bf16, D = 128, pages of 64 rows).
 //
 // Token t of sequence b (cu_seqlens[b] <= t < cu_seqlens[b+1]) sits at position p = seq_lens[b] - cu_seqlens[b+1] + t and
 // sees the cached rows j <= p, its own among them:  out[t, h] = sum_j softmax_j(q[t, h] . k_j * scale) v_j, query head h
-// reading kv head h / (Hq / Hkv).  One warp per (token, query head), one pass over the rows with the running maximum and
-// sum of the softmax in fp32.
+// reading kv head h / (Hq / Hkv).  One pass over the rows with the running maximum and sum of the softmax in fp32.
+//
+// Tiles.  The `group` query heads of a kv head share its K and V, so a tile's 128 rows are floor(128 / group) tokens times
+// group heads (row = token * group + head).  Tiles run over sequence, kv head, chunk of tokens; each has a number of KV
+// blocks of 128 rows (two pages) that follows from the device-side lengths.  The blocks of all tiles form one line, which
+// is cut into equal ranges, one per CTA: a few drafted tokens over one long cache keep every SM as busy as a long prompt
+// does, and all CTAs end together, whatever the lengths.  A range that covers a whole tile writes its output; the (at
+// most two) tiles that a CTA has in part leave un-normalised fp32 partials (o, m, l), which a second kernel joins in
+// the order of the line, so results do not depend on timing.
+//
+// Inside a CTA the blocks of its ranges form one stream, numbered g = 0, 1, 2, ..., that does not stop at tile borders:
+//
+//   S(g) = Q K(g)^T      8 x tcgen05.mma 128x128x16, both operands in shared memory, into TMEM buffer g % 3
+//   softmax(g)           warpgroup g & 1 (thread = row = TMEM lane): scores to registers, row maximum, p = 2^(s - m),
+//                        P(g) as packed 16-bit over the first 64 columns of the same TMEM buffer
+//   O += P(g) V(g)       8 x tcgen05.mma 128x128x16 with P read from TMEM, O in TMEM columns 384..511
+//
+//   warps 0-3 / 4-7  softmax of even / odd blocks      warps 8-11   epilogue
+//   warp 12, 15      TMA producers: Q and K (and the list of tiles); V (warp 15 also allocates the 512 TMEM columns)
+//   warp 13, 14      issuers of the score products and of the PV products (one lane each)
+//
+// P is rounded to the storage type because the second product takes both operands in one 16-bit type; the row sum adds
+// the unrounded values.  The running maximum passes between the warpgroups through shared memory, O is rescaled only when
+// it grows by more than 2^8 (a weight is then at most 2^8, far inside fp16).
+//
+// What is masked.  A table entry that is not needed or not in the pool becomes a coordinate outside the tensor map, which
+// TMA fills with zeros; nothing outside the pool is addressed.  Scores of hidden columns are replaced, not added to, so K
+// may hold anything there.  V may not, since 0 * NaN is NaN: in the blocks that some row of the tile does not see
+// whole, the softmax warps clear V rows behind the sequence's end in shared memory, and look for infinities and NaN in the
+// rows that only some of the tile's rows see.  Such a value is replaced by 0 and noted; the epilogue makes it a NaN in
+// exactly those rows that see it.
+//
+// Every wait is bounded; on expiry the CTA records a code in the status words and unwinds.
+#include <cuda.h>
+
 #include "nb200_common.cuh"
+#include "sm100_primitives.cuh"
+#include "tma_host.cuh"
 
 namespace nb200 {
 namespace {
 
-constexpr int kPageRows = 64;
-constexpr int kD = 128;
-constexpr int kErrTable = 22;
+using namespace sm100;
 
+constexpr int kPageRows = 64;
+constexpr int kBM = 128;
+constexpr int kBN = 128;                        // rows of a KV block: two pages
+constexpr int kD = 128;
+constexpr int kThreads = 512;
+constexpr int kTileBytes = 128 * kD * 2;        // 32 KB: two halves of 64 columns, 16 KB each
+constexpr int kBox = kTileBytes / 2;
+constexpr int kPageBox = kPageRows * 128;       // one page's half: 8 KB
+constexpr int kSBufs = 3;
+constexpr int kTmemCols = 512;                  // S/P 0 | S/P 1 | S/P 2 | O, 128 columns each
+constexpr int kTmemO = 384;
+constexpr float kRescaleThreshold = 8.0f;
+constexpr int kSched = 16;                      // ring of tile descriptors handed from the K producer to the other roles
+constexpr int kMaxCtas = 160;                   // CTAs that the workspace has room for
+
+enum : int { kErrProducer = 41, kErrMma = 42, kErrSoftmax = 43, kErrEpilogue = 44, kErrTable = 22, kErrSlot = 23 };
+
+// Part of a tile that one CTA works on.
+struct Segment {
+  int more;                  // 0: the list ends here
+  int b, kvh;
+  int tok0, ntok;            // first row of the batch, tokens
+  int pos0;                  // position of the first token
+  int len;                   // rows of the sequence's cache
+  int blk0, nblk;            // KV blocks
+  int slot;                  // -1: the whole tile; 0 / 1: partial that ends / begins a tile
+};
+// Tile that begins in a CTA and goes on in the next ones.
+struct Owner {
+  int parts;                 // 0: none
+  int kvh, tok0, ntok;
+};
 struct Args {
-  const void *q, *k_pages, *v_pages;
-  void *out;
   const int *block_table, *cu_seqlens, *seq_lens;
-  long long q_t, q_h, out_t, out_h;
-  int T, B, Hq, Hkv, num_pages, max_pages;
+  uint16_t *out;
+  long long out_t, out_h;
+  int T, B, Hkv, group, tok_tile, num_pages, max_pages;
   float scale_log2;
+  float *part_o;             // [kMaxCtas][2][128][128]
+  float2 *part_ml;           // [kMaxCtas][2][128]
+  Owner *owners;             // [kMaxCtas]
   int *status;
 };
+constexpr size_t kPartO = static_cast<size_t>(kMaxCtas) * 2 * kBM * kD * sizeof(float);
+constexpr size_t kPartMl = static_cast<size_t>(kMaxCtas) * 2 * kBM * sizeof(float2);
 
-template <int DT> __global__ void __launch_bounds__(32) attn_paged_kernel(const Args a) {
-  const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-  int below = 0;
-  for (int i = lane; i <= a.B; i += 32) below += a.cu_seqlens[i] <= t;
-  const int b = __reduce_add_sync(0xffffffffu, below) - 1;
-  if (b < 0 || b >= a.B || t < a.cu_seqlens[b] || t >= a.cu_seqlens[b + 1]) return;
-  const long long p = static_cast<long long>(a.seq_lens[b]) - a.cu_seqlens[b + 1] + t;
-  const long long last = min(p, min(static_cast<long long>(a.seq_lens[b]), static_cast<long long>(a.max_pages) * kPageRows) - 1);
-  float2 q01 = unpack2<DT>(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.q) + t * a.q_t + h * a.q_h)[lane].x);
-  float2 q23 = unpack2<DT>(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.q) + t * a.q_t + h * a.q_h)[lane].y);
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  const int kv = h / (a.Hq / a.Hkv);
-  bool bad = false;
-  for (long long j = 0; j <= last; ++j) {
-    const int page = a.block_table[static_cast<long long>(b) * a.max_pages + j / kPageRows];
-    if (page < 0 || page >= a.num_pages) {
-      if (a.status && lane == 0 && atomicCAS(a.status, 0, kErrTable) == 0) {
-        a.status[1] = static_cast<int>(blockIdx.x);
-        a.status[2] = page;
-        a.status[3] = lane;
-      }
-      bad = true;
-      break;
-    }
-    const long long row = ((static_cast<long long>(page) * a.Hkv + kv) * kPageRows + j % kPageRows) * kD;
-    const uint2 kw = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.k_pages) + row)[lane];
-    const uint2 vw = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.v_pages) + row)[lane];
-    const float2 k01 = unpack2<DT>(kw.x), k23 = unpack2<DT>(kw.y), v01 = unpack2<DT>(vw.x), v23 = unpack2<DT>(vw.y);
-    float x = q01.x * k01.x + q01.y * k01.y + q23.x * k23.x + q23.y * k23.y;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-    x *= a.scale_log2;
-    const float m_new = fmaxf(m, x), f = m == m_new ? 1.f : ex2(m - m_new), w = ex2(x - m_new);
-    m = m_new;
-    l = l * f + w;
-    o[0] = o[0] * f + w * v01.x;
-    o[1] = o[1] * f + w * v01.y;
-    o[2] = o[2] * f + w * v23.x;
-    o[3] = o[3] * f + w * v23.y;
+struct Shared {
+  uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full[kSBufs], p_full[kSBufs], pv_done[kSBufs];
+  uint64_t o_full, o_free, m_ready[2], lm_ready, lm_free;
+  uint64_t sched_full[kSched];
+  unsigned long long taint[2][kD];   // per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is not finite)
+  long long scan[kThreads / 32];
+  long long first_block, last_block, total;
+  Segment seg[kSched];
+  int start_b, start_h, start_j, start_blk;
+  int taint_any[2];                  // tile number + 1
+  uint32_t tmem_base;
+  int abort_flag;
+  int skip;
+  float mslot[2][kBM];               // running maximum decided by block g, slot g & 1
+  float lm[2][kBM][2];               // per warpgroup: (maximum last used, partial row sum) of the finished tile
+};
+constexpr int kSmemBytes = 6 * kTileBytes + 1024 + static_cast<int>(sizeof(Shared));
+
+__device__ __forceinline__ void report(int *status, int code, int detail) {
+  if (status && atomicCAS(status, 0, code) == 0) {
+    status[1] = static_cast<int>(blockIdx.x);
+    status[2] = detail;
+    status[3] = static_cast<int>(threadIdx.x);
   }
-  const float inv = bad ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);   // a row that sees nothing is 0
-  reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + t * a.out_t + h * a.out_h)[lane] =
-      make_uint2(pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv));
+}
+
+// New tokens of a sequence, where they sit and what there is to see.  Clamped, so that no device-side value leads out of
+// the tensors: rows stay inside [0, T), positions inside [-T - 1, len].
+struct Seq {
+  int first, n, pos, len;
+};
+__device__ __forceinline__ Seq seq_of(const Args &a, int b) {
+  const int c0 = a.cu_seqlens[b], c1 = a.cu_seqlens[b + 1], len = a.seq_lens[b];
+  Seq s;
+  s.first = max(c0, 0);
+  s.n = max(min(c1, a.T) - s.first, 0);
+  s.len = min(max(len, 0), a.max_pages * kPageRows);
+  const long long pos = static_cast<long long>(len) - c1 + s.first;
+  s.pos = static_cast<int>(max(min(pos, static_cast<long long>(s.len)), -static_cast<long long>(a.T) - 1));
+  return s;
+}
+// KV blocks of the tile that starts at token j0 of the sequence: what its last token sees, at least one.
+__device__ __forceinline__ int tile_blocks(const Seq &s, int j0, int tok_tile) {
+  const int sees = min(s.pos + min(s.n, j0 + tok_tile), s.len);
+  return sees <= 0 ? 1 : (sees + kBN - 1) / kBN;
+}
+__device__ __forceinline__ long long seq_blocks(const Seq &s, int tok_tile) {
+  long long sum = 0;
+  for (int j0 = 0; j0 < s.n; j0 += tok_tile) sum += tile_blocks(s, j0, tok_tile);
+  return sum;
+}
+
+// fma(x, 0, acc) on packed 16-bit pairs: stays 0 while every x is finite, becomes NaN for good otherwise.
+template <int DT> __device__ __forceinline__ uint32_t finite_probe(uint32_t x, uint32_t acc) {
+  uint32_t r;
+  if constexpr (DT == NB200_BF16)
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  else
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
+  return r;
+}
+template <int DT> __device__ __forceinline__ bool not_finite16(uint32_t h) {
+  return DT == NB200_BF16 ? (h & 0x7f80u) == 0x7f80u : (h & 0x7c00u) == 0x7c00u;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                  const __grid_constant__ CUtensorMap tm_v, const Args a) {
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char *smem = smem_raw + (base - raw);
+  const uint32_t sQ = base;                                   // buffer n & 1 of tile n
+  const uint32_t sK = base + 2 * kTileBytes;                  // stage g & 1
+  const uint32_t sV = base + 4 * kTileBytes;
+  Shared *sh = reinterpret_cast<Shared *>(smem + 6 * kTileBytes);
+  volatile int *abort_flag = &sh->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
+  if (threadIdx.x == 0) {
+    sh->abort_flag = 0;
+    const int code = a.status ? *reinterpret_cast<volatile int *>(a.status) : 0;
+    sh->skip = (code != 0 && code != kErrTable && code != kErrSlot) ? 1 : 0;   // an expired wait, not refused data
+    a.owners[blockIdx.x].parts = 0;
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&sh->q_full[b]), 1);
+      mbar_init(smem_u32(&sh->q_empty[b]), 1);
+      mbar_init(smem_u32(&sh->k_full[b]), 1);
+      mbar_init(smem_u32(&sh->k_empty[b]), 1);
+      mbar_init(smem_u32(&sh->v_full[b]), 1);
+      mbar_init(smem_u32(&sh->v_empty[b]), 1);
+      mbar_init(smem_u32(&sh->m_ready[b]), 128);
+      sh->taint_any[b] = 0;
+    }
+    for (int b = 0; b < kSBufs; ++b) {
+      mbar_init(smem_u32(&sh->s_full[b]), 1);
+      mbar_init(smem_u32(&sh->p_full[b]), 128);
+      mbar_init(smem_u32(&sh->pv_done[b]), 1);
+    }
+    mbar_init(smem_u32(&sh->o_full), 1);
+    mbar_init(smem_u32(&sh->o_free), 128);
+    mbar_init(smem_u32(&sh->lm_ready), 256);
+    mbar_init(smem_u32(&sh->lm_free), 128);
+    for (int b = 0; b < kSched; ++b) mbar_init(smem_u32(&sh->sched_full[b]), 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (threadIdx.x < 2 * kD) sh->taint[threadIdx.x / kD][threadIdx.x % kD] = 0;
+
+  // ---- the CTA's range of the line of blocks: a scan over the sequences' block counts, a thread per sequence ----
+  auto scan = [&](int b0, long long &running, long long &before) -> long long {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const long long mine = b < a.B ? seq_blocks(seq_of(a, b), a.tok_tile) * a.Hkv : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    __syncthreads();
+    if (lane == 31) sh->scan[warp] = incl;
+    __syncthreads();
+    before = running + incl - mine;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += sh->scan[w];
+      running += sh->scan[w];
+    }
+    return mine;
+  };
+  long long total = 0, before = 0, mine = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) mine = scan(b0, total, before);
+  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+  if (sh->skip || static_cast<int>(blockIdx.x) >= ctas) return;   // the same for every thread of the CTA
+  const long long r0 = total * blockIdx.x / ctas, r1 = total * (blockIdx.x + 1) / ctas;
+  auto locate = [&](int b) {   // the thread whose sequence holds block r0 finds kv head, tile and block in it
+    if (before > r0 || r0 >= before + mine) return;
+    const Seq s = seq_of(a, b);
+    const long long per_head = mine / a.Hkv;
+    long long rem = r0 - before;
+    sh->start_b = b;
+    sh->start_h = static_cast<int>(rem / per_head);
+    rem %= per_head;
+    int j0 = 0;
+    for (int n; rem >= (n = tile_blocks(s, j0, a.tok_tile)); j0 += a.tok_tile) rem -= n;
+    sh->start_j = j0;
+    sh->start_blk = static_cast<int>(rem);
+  };
+  if (a.B <= kThreads) {
+    locate(threadIdx.x);
+  } else {
+    long long running = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+      mine = scan(b0, running, before);
+      locate(b0 + static_cast<int>(threadIdx.x));
+    }
+  }
+
+  if (warp == 15) {
+    tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 12 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh->tmem_base;
+
+  const uint32_t b_q_full = smem_u32(&sh->q_full[0]), b_q_empty = smem_u32(&sh->q_empty[0]),
+                 b_k_full = smem_u32(&sh->k_full[0]), b_k_empty = smem_u32(&sh->k_empty[0]),
+                 b_v_full = smem_u32(&sh->v_full[0]), b_v_empty = smem_u32(&sh->v_empty[0]),
+                 b_s_full = smem_u32(&sh->s_full[0]), b_p_full = smem_u32(&sh->p_full[0]),
+                 b_pv_done = smem_u32(&sh->pv_done[0]), b_o_full = smem_u32(&sh->o_full),
+                 b_o_free = smem_u32(&sh->o_free), b_m_ready = smem_u32(&sh->m_ready[0]),
+                 b_lm_ready = smem_u32(&sh->lm_ready), b_lm_free = smem_u32(&sh->lm_free),
+                 b_sched = smem_u32(&sh->sched_full[0]);  // element i at + 8 * i
+
+  // The K producer lists the CTA's tiles in a ring that every other role reads.  The roles are never more than 7 tiles
+  // apart (2 Q buffers, 3 score buffers, one O), so 16 slots need no "empty" barrier.  Null: an expired wait.
+  auto segment_at = [&](int n) -> const volatile Segment * {
+    if (!mbar_wait(b_sched + 8 * (n % kSched), (n / kSched) & 1, abort_flag)) return nullptr;
+    return &sh->seg[n % kSched];
+  };
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    if (warp == 12 || warp == 15) {
+      // ================================ TMA producers ================================
+      // warp 12: the list of tiles, Q of every tile and the K blocks; warp 15: the V blocks.  Lane i reads the table
+      // entry of page i of the next 16 blocks, lane 0 waits and issues.
+      const bool is_k = warp == 12;
+      const CUtensorMap *tm = is_k ? &tm_k : &tm_v;
+      const uint32_t s_dst = is_k ? sK : sV, b_full = is_k ? b_k_full : b_v_full, b_empty = is_k ? b_k_empty : b_v_empty;
+      const int outside = a.num_pages * a.Hkv;             // a slice that the tensor map does not have: zeros
+      const int q_bytes = a.group * a.tok_tile * 256;
+      int sb = sh->start_b, shd = sh->start_h, sj = sh->start_j, sblk = sh->start_blk;   // the scheduler's place
+      long long at = r0;
+      bool ok = true;
+      int g = 0, issued = 0, q_issued = 0;
+      for (int n = 0; ok; ++n) {
+        if (is_k) {
+          if (lane == 0) {
+            Segment w{};
+            if (at < r1) {
+              Seq s = seq_of(a, sb);
+              if (sj >= s.n) {                             // on to the next kv head, or sequence with new tokens
+                sj = 0;
+                if (++shd == a.Hkv) {
+                  shd = 0;
+                  do s = seq_of(a, ++sb); while (s.n == 0 && sb < a.B - 1);   // at < r1: there is one
+                }
+              }
+              const int blocks = tile_blocks(s, sj, a.tok_tile);
+              const int take = static_cast<int>(min(static_cast<long long>(blocks - sblk), r1 - at));
+              w.more = 1;
+              w.b = sb, w.kvh = shd;
+              w.tok0 = s.first + sj, w.ntok = min(a.tok_tile, s.n - sj);
+              w.pos0 = s.pos + sj, w.len = s.len;
+              w.blk0 = sblk, w.nblk = take;
+              w.slot = take == blocks ? -1 : (sblk > 0 ? 0 : 1);
+              if (w.slot == 1) {                           // goes on in the CTAs up to the one that has its last block
+                const long long end = at + blocks;
+                const int last = static_cast<int>((end * ctas + total - 1) / total) - 1;
+                a.owners[blockIdx.x] = Owner{last - static_cast<int>(blockIdx.x) + 1, w.kvh, w.tok0, w.ntok};
+              }
+              at += take;
+              sblk += take;
+              if (sblk == blocks) {
+                sblk = 0;
+                sj += a.tok_tile;
+              }
+            }
+            sh->seg[n % kSched] = w;
+            mbar_arrive(b_sched + 8 * (n % kSched));
+          }
+          __syncwarp();
+        }
+        const volatile Segment *seg = segment_at(n);
+        if (!__all_sync(0xffffffffu, seg != nullptr)) {
+          if (lane == 0) report(a.status, kErrProducer, -1000 - n);
+          ok = false;
+          break;
+        }
+        if (!seg->more) break;
+        const int kvh = seg->kvh, blk0 = seg->blk0, nblk = seg->nblk;
+        const int pages = min((seg->len + kPageRows - 1) / kPageRows, 2 * (blk0 + nblk));   // needed here
+        const int *table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
+        if (is_k && lane == 0) {
+          ok = mbar_wait(b_q_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag);
+          if (!ok) {
+            report(a.status, kErrProducer, -1 - n);
+          } else {
+            mbar_arrive_expect_tx(b_q_full + 8 * (n & 1), q_bytes);
+            tma_load_3d(sQ + (n & 1) * kTileBytes, &tm_q, 0, kvh * a.group, seg->tok0, b_q_full + 8 * (n & 1));
+            tma_load_3d(sQ + (n & 1) * kTileBytes + kBox, &tm_q, 64, kvh * a.group, seg->tok0, b_q_full + 8 * (n & 1));
+            ++q_issued;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        auto slice_of = [&](int j) -> int {                // of page (2 * (blk0 + j) + lane): its slice of the pool's map
+          const int page = 2 * (blk0 + j) + lane;
+          if (page >= pages) return outside;
+          const int e = table[page];
+          if (e >= 0 && e < a.num_pages) return e * a.Hkv + kvh;
+          if (is_k) report(a.status, kErrTable, e);
+          return outside;
+        };
+        int next = slice_of(0);
+        for (int j0 = 0; j0 < nblk && ok; j0 += 16) {
+          const int slices = next;
+          if (j0 + 16 < nblk) next = slice_of(j0 + 16);
+          for (int j = j0; j < min(nblk, j0 + 16) && ok; ++j, ++g) {
+            const int s0 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0)), s1 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0) + 1);
+            if (lane == 0) {
+              const int st = g & 1;
+              ok = mbar_wait(b_empty + 8 * st, ((g >> 1) & 1) ^ 1, abort_flag);
+              if (!ok) {
+                report(a.status, kErrProducer, 2 * g + (is_k ? 0 : 1));
+              } else {
+                const uint32_t dst = s_dst + st * kTileBytes, bar = b_full + 8 * st;
+                mbar_arrive_expect_tx(bar, kTileBytes);
+                tma_load_3d(dst, tm, 0, 0, s0, bar);
+                tma_load_3d(dst + kPageBox, tm, 0, 0, s1, bar);
+                tma_load_3d(dst + kBox, tm, 64, 0, s0, bar);
+                tma_load_3d(dst + kBox + kPageBox, tm, 64, 0, s1, bar);
+                ++issued;
+              }
+            }
+            ok = __all_sync(0xffffffffu, ok);
+          }
+        }
+      }
+      if (!ok && lane == 0) {
+        // Unwinding: let the copies already in flight land before the CTA's shared memory goes away.
+        for (int spin = 0; spin < 100000; ++spin) {
+          bool done = true;
+          for (int n = 0; n < 2; ++n) {
+            const int jg = issued - 1 - n, jq = q_issued - 1 - n;
+            if (jg >= 0) done = done && mbar_try_wait(b_full + 8 * (jg & 1), (jg >> 1) & 1);
+            if (jq >= 0) done = done && mbar_try_wait(b_q_full + 8 * (jq & 1), (jq >> 1) & 1);
+          }
+          if (done) break;
+          __nanosleep(100);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 13) {
+      // ================================ score-product issuer ==================================
+      // A thread of its own for each of the two products: issuing one and testing barriers for the other in between
+      // does not keep the pipe fed.  S(g) goes into the buffer P(g-3) was read from: wait for that PV product first.
+      if (lane == 0) {
+        constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
+        constexpr uint32_t idesc_qk = umma_idesc_f16(fmt, 0, kBM, kBN);
+        const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
+        uint32_t dq_lo[kD / 16], dk_lo[kD / 16];   // buffer / stage 1 is kStageStep further
+        constexpr uint32_t kStageStep = kTileBytes >> 4;
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32;
+          dq_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sQ + off, 16, 1024));
+          dk_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sK + off, 16, 1024));
+        }
+        bool ok = true;
+        int g = 0;
+        for (int n = 0; ok; ++n) {
+          const volatile Segment *seg = segment_at(n);
+          if (!seg) { report(a.status, kErrMma, -1000 - n); break; }
+          if (!seg->more) break;
+          const int nblk = seg->nblk;
+          ok = mbar_wait(b_q_full + 8 * (n & 1), (n >> 1) & 1, abort_flag);
+          if (!ok) { report(a.status, kErrMma, -1 - n); break; }
+          const uint32_t q_step = (n & 1) * kStageStep;
+          for (int j = 0; j < nblk && ok; ++j, ++g) {
+            const int sb = g % kSBufs;
+            ok = mbar_wait(b_k_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
+            if (!ok) { report(a.status, kErrMma, 4 * g); break; }
+            if (g >= kSBufs) {
+              ok = mbar_wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1, abort_flag);
+              if (!ok) { report(a.status, kErrMma, 4 * g + 1); break; }
+            }
+            tc_fence_after();
+            const uint32_t d_tmem = tmem + sb * 128, k_step = (g & 1) * kStageStep;
+#pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) umma_ss_lo(d_tmem, dq_lo[kk] + q_step, dk_lo[kk] + k_step, d_hi, idesc_qk, kk > 0);
+            umma_commit(b_s_full + 8 * sb);
+            umma_commit(b_k_empty + 8 * (g & 1));
+          }
+          if (ok) umma_commit(b_q_empty + 8 * (n & 1));
+        }
+      }
+      __syncwarp();
+    } else {
+      // ================================ PV-product issuer ==================================
+      if (lane == 0) {
+        constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
+        constexpr uint32_t idesc_pv = umma_idesc_f16(fmt, 1, kBM, kD);
+        // V is MN-major: 16 kv rows = 2 KB, the two 64-column halves kBox apart
+        const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
+        uint32_t dv_lo[kBN / 16];
+        constexpr uint32_t kStageStep = kTileBytes >> 4;
+#pragma unroll
+        for (int kk = 0; kk < kBN / 16; ++kk) dv_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sV + kk * 2048, kBox, 1024));
+        bool ok = true;
+        int g = 0;
+        for (int n = 0; ok; ++n) {
+          const volatile Segment *seg = segment_at(n);
+          if (!seg) { report(a.status, kErrMma, -1000 - n); break; }
+          if (!seg->more) break;
+          const int nblk = seg->nblk;
+          for (int j = 0; j < nblk && ok; ++j, ++g) {
+            const int sb = g % kSBufs;
+            ok = mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
+            if (!ok) { report(a.status, kErrMma, 4 * g + 2); break; }
+            if (j == 0 && n > 0) {   // the epilogue of the previous tile has read O
+              ok = mbar_wait(b_o_free, (n - 1) & 1, abort_flag);
+              if (!ok) { report(a.status, kErrMma, 4 * g + 3); break; }
+            }
+            ok = mbar_wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1, abort_flag);
+            if (!ok) { report(a.status, kErrMma, 4 * g + 3); break; }
+            tc_fence_after();
+            const uint32_t p_tmem = tmem + sb * 128, v_step = (g & 1) * kStageStep;
+#pragma unroll
+            for (int kk = 0; kk < kBN / 16; ++kk)   // P: 16 packed 16-bit values = 8 TMEM columns per product
+              umma_ts_lo(tmem + kTmemO, p_tmem + kk * 8, dv_lo[kk] + v_step, d_hi, idesc_pv, (kk > 0 || j > 0) ? 1u : 0u);
+            umma_commit(b_pv_done + 8 * sb);
+            umma_commit(b_v_empty + 8 * (g & 1));
+            if (j + 1 == nblk) umma_commit(b_o_full);
+          }
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp >= 8) {
+    // ================================ epilogue: O / l -> out, or (O, m, l) -> workspace ==========================
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t tO = tmem + kTmemO + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int tok = r / a.group, head = r % a.group;
+    for (int n = 0;; ++n) {
+      const volatile Segment *seg = segment_at(n);
+      if (!__all_sync(0xffffffffu, seg != nullptr)) { report(a.status, kErrEpilogue, -1000 - n); break; }
+      if (!seg->more) break;
+      const int slot = seg->slot;
+      const bool row_exists = tok < seg->ntok;
+      const int last_seen = min(seg->pos0 + tok, seg->len - 1);
+      uint16_t *dst = a.out + static_cast<long long>(seg->tok0 + tok) * a.out_t + static_cast<long long>(seg->kvh * a.group + head) * a.out_h;
+      // a table entry outside the pool among the pages read: NaN instead of a sum that lacks them
+      bool bad = false;
+      {
+        const int *table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
+        const int end = min(2 * (seg->blk0 + seg->nblk), (seg->len + kPageRows - 1) / kPageRows);
+        for (int p = 2 * seg->blk0 + lane; p < end; p += 32) bad = bad || static_cast<unsigned>(table[p]) >= static_cast<unsigned>(a.num_pages);
+        bad = __any_sync(0xffffffffu, bad);
+      }
+      bool ok = __all_sync(0xffffffffu, mbar_wait(b_lm_ready, n & 1, abort_flag));
+      if (!ok) { report(a.status, kErrEpilogue, 2 * n); break; }
+      const float m0 = sh->lm[0][r][0], l0 = sh->lm[0][r][1], m1 = sh->lm[1][r][0], l1 = sh->lm[1][r][1];
+      const bool tainted = *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) == n + 1;
+      if (!tainted) mbar_arrive(b_lm_free);   // else the notes of this tile are still to be read
+      const float mf = fmaxf(m0, m1);         // the running maximum never decreases: the later one is the larger
+      float l = (l0 == 0.f ? 0.f : l0 * ex2(m0 - mf)) + (l1 == 0.f ? 0.f : l1 * ex2(m1 - mf));
+      const bool empty = l == 0.f;            // no visible row (in this part): 0, whatever the products hold
+      if (bad) l = __int_as_float(0x7fffffff);
+      const float inv = empty && !bad ? 0.f : (slot < 0 ? 1.f / l : 1.f);
+      float *po = nullptr;
+      if (slot >= 0) {
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + r;
+        po = a.part_o + pr * kD;
+        if (row_exists) a.part_ml[pr] = make_float2(mf, l);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(b_o_full, n & 1, abort_flag));
+      if (!ok) { report(a.status, kErrEpilogue, 2 * n + 1); break; }
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
+        tmem_wait_ld();
+        if (c == kD / 32 - 1) {   // O is in registers: the next tile may overwrite it
+          tc_fence_before();
+          mbar_arrive(b_o_free);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[k]) * inv);
+        if (tainted) {
+#pragma unroll 1
+          for (int k = 0; k < 32; ++k) {
+            const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c * 32 + k]);
+            if (static_cast<int>(note >> 32) == n + 1 && static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) <= last_seen) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (i == k) o[i] = 0x7fffffffu;
+            }
+          }
+        }
+        if (row_exists) {
+          if (slot < 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 w;
+              w.x = pack2<DT>(__uint_as_float(o[8 * k + 0]), __uint_as_float(o[8 * k + 1]));
+              w.y = pack2<DT>(__uint_as_float(o[8 * k + 2]), __uint_as_float(o[8 * k + 3]));
+              w.z = pack2<DT>(__uint_as_float(o[8 * k + 4]), __uint_as_float(o[8 * k + 5]));
+              w.w = pack2<DT>(__uint_as_float(o[8 * k + 6]), __uint_as_float(o[8 * k + 7]));
+              *reinterpret_cast<uint4 *>(dst + c * 32 + k * 8) = w;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              reinterpret_cast<uint4 *>(po + c * 32)[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        }
+        __syncwarp();   // the next load from TMEM is one for the whole warp
+      }
+      if (tainted) mbar_arrive(b_lm_free);
+    }
+  } else {
+    // ================================ softmax: warpgroup w takes the blocks g with g & 1 == w ================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    const int w = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;                     // row in the tile == TMEM lane
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tO = tmem + kTmemO + lane_addr;
+    const int tok = r / a.group;
+    int n = 0, g0 = 0;
+    bool ok = true, more = true;
+    int nblk = 0, blk0 = 0, pos0 = 0, len = 0, ntok = 0;
+    auto read_segment = [&]() {
+      const volatile Segment *seg = segment_at(n);
+      ok = __all_sync(0xffffffffu, seg != nullptr);
+      if (!ok) {
+        report(a.status, kErrSoftmax, -1000 - n);
+        return;
+      }
+      more = seg->more;
+      nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
+    };
+    read_segment();
+    float m_mine = -INFINITY, l = 0.f;
+    for (int g = w; ok; g += 2) {
+      // tiles that end before block g: hand (maximum, partial sum) to the epilogue and move on
+      while (more && g >= g0 + nblk) {
+        if (n > 0) {   // the epilogue has read the previous tile's values
+          ok = __all_sync(0xffffffffu, mbar_wait(b_lm_free, (n - 1) & 1, abort_flag));
+          if (!ok) { report(a.status, kErrSoftmax, -1 - n); break; }
+        }
+        sh->lm[w][r][0] = m_mine;
+        sh->lm[w][r][1] = l;
+        mbar_arrive(b_lm_ready);
+        m_mine = -INFINITY;
+        l = 0.f;
+        g0 += nblk;
+        ++n;
+        read_segment();
+        if (!ok) break;
+      }
+      if (!ok || !more) break;
+      const int j = g - g0;
+      const int sb = g % kSBufs;
+      const int col0 = (blk0 + j) * kBN;                       // cache row of the block's first column
+      const uint32_t tS = tmem + sb * 128 + lane_addr;
+      ok = __all_sync(0xffffffffu, mbar_wait(b_s_full + 8 * sb, (g / kSBufs) & 1, abort_flag));
+      if (!ok) { report(a.status, kErrSoftmax, g); break; }
+      tc_fence_after();
+      float m_prev = -INFINITY;
+      if (g > 0) {
+        // block g-1 has decided on its maximum (and, before that, has read the slot this block will overwrite)
+        ok = __all_sync(0xffffffffu, mbar_wait(b_m_ready + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag));
+        if (!ok) { report(a.status, kErrSoftmax, 1000 + g); break; }
+        if (j > 0) m_prev = sh->mslot[(g - 1) & 1][r];
+      }
+      // column c of the block is seen by this row iff c <= vis
+      const int vis = tok < ntok ? min(pos0 + tok, len - 1) - col0 : -1;
+      const bool warp_works = __any_sync(0xffffffffu, vis >= 0);   // else P may hold anything: no row of the warp is used, or none sees the block
+      float m_new = m_prev;
+      if (!warp_works) {
+        // a row that sees nothing here still must not take anything from the products: P = 0
+        sh->mslot[g & 1][r] = m_prev;
+        mbar_arrive(b_m_ready + 8 * (g & 1));
+        const uint32_t zero[16] = {};
+#pragma unroll
+        for (int c = 0; c < kBN / 32; ++c) tmem_st16(tS + c * 16, zero);
+      } else {
+        uint32_t v[kBN];
+        tmem_ld32p(tS, v);
+        tmem_ld32p(tS + 32, v + 32);
+        tmem_ld32p(tS + 64, v + 64);
+        tmem_ld32p(tS + 96, v + 96);
+        tmem_wait_ld();
+        if (vis < kBN - 1) {
+#pragma unroll
+          for (int c = 0; c < kBN; ++c) v[c] = (c > vis) ? 0xff800000u : v[c];
+        }
+        // ---- row maximum: eight chains of three-input maxima ----
+        float mc[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          mc[c] = max3(__uint_as_float(v[c * 16]), __uint_as_float(v[c * 16 + 1]), __uint_as_float(v[c * 16 + 2]));
+#pragma unroll
+        for (int k = 3; k + 1 < 16; k += 2) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            mc[c] = max3(mc[c], __uint_as_float(v[c * 16 + k]), __uint_as_float(v[c * 16 + k + 1]));
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mc[c] = fmaxf(mc[c], __uint_as_float(v[c * 16 + 15]));
+        const float mx = fmaxf(max3(mc[0], mc[1], mc[2]), fmaxf(max3(mc[3], mc[4], mc[5]), fmaxf(mc[6], mc[7])));
+        const float m_blk = mx * a.scale_log2;                   // -inf if the row sees nothing of this block
+        // ---- the maximum to use: the one block g-1 decided on, unless this block exceeds it by more than 2^8 ----
+        const bool need = j > 0 && m_blk > m_prev + kRescaleThreshold;
+        m_new = (j == 0 || need) ? m_blk : m_prev;
+        sh->mslot[g & 1][r] = m_new;
+        mbar_arrive(b_m_ready + 8 * (g & 1));
+        if (__any_sync(0xffffffffu, need)) {
+          // O must hold every product up to block g-1 and none may be in flight
+          ok = __all_sync(0xffffffffu, mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag));
+          if (!ok) { report(a.status, kErrSoftmax, 2000 + g); break; }
+          tc_fence_after();
+          const float f = need ? ex2(m_prev - m_blk) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < kD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(tO + c * 16, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st16(tO + c * 16, o);
+          }
+          tmem_wait_st();
+        }
+        if (m_mine != m_new) {   // bring the partial sum to the new maximum (2^(-inf) = 0 on the first block)
+          l *= ex2(m_mine - m_new);
+          m_mine = m_new;
+        }
+        // ---- p = 2^(s*scale - m), row sum, pack to 16 bit; P overwrites columns 0..63 of S ----
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;    // nothing seen so far: every p is 2^(-inf) = 0
+        const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
+        uint64_t lsum2 = f2_pack(0.f, 0.f);
+#pragma unroll
+        for (int c = 0; c < kBN / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t x2 = f2_fma(
+                f2_pack(__uint_as_float(v[c * 32 + 2 * k]), __uint_as_float(v[c * 32 + 2 * k + 1])), c2, nm2);
+            const float2 x = f2_unpack(x2);
+            const float p0 = ex2(x.x), p1 = ex2(x.y);
+            lsum2 = f2_add(lsum2, f2_pack(p0, p1));
+            pk[k] = pack2<DT>(p0, p1);
+          }
+          tmem_st16(tS + c * 16, pk);
+        }
+        const float2 ls = f2_unpack(lsum2);
+        l += ls.x + ls.y;
+      }
+      // ---- V rows that not every row of the tile sees ----
+      const int lo = max(pos0 + 1 - col0, 0), hi = max(len - col0, 0);   // from lo on the first token sees nothing; the cache ends at hi
+      if (min(lo, hi) < kBN) {
+        // V(g-2), in the same buffer, must have come and gone first: the barrier tells two phases apart, not three
+        if (g >= 2) ok = mbar_wait(b_pv_done + 8 * ((g - 2) % kSBufs), ((g - 2) / kSBufs) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok && mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag));
+        if (!ok) { report(a.status, kErrSoftmax, 3000 + g); break; }
+        unsigned char *row = smem + 4 * kTileBytes + (g & 1) * kTileBytes + r * 128;   // thread = row of V here
+        if (r >= hi) {
+#pragma unroll
+          for (int c = 0; c < 16; ++c)
+            *reinterpret_cast<uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        } else if (r >= lo) {
+          uint32_t probe = 0u;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16);
+            probe = finite_probe<DT>(x.x, probe);
+            probe = finite_probe<DT>(x.y, probe);
+            probe = finite_probe<DT>(x.z, probe);
+            probe = finite_probe<DT>(x.w, probe);
+          }
+          if (not_finite16<DT>(probe & 0xffffu) || not_finite16<DT>(probe >> 16)) {
+#pragma unroll 1
+            for (int c = 0; c < kD; ++c) {   // column c: 16-byte piece (c / 8) % 8 of its half, swizzled with the row
+              uint16_t *x = reinterpret_cast<uint16_t *>(row + (c >> 6) * kBox + (((c >> 3) ^ r) & 7) * 16) + (c & 7);
+              if (not_finite16<DT>(*x)) {
+                *x = 0;
+                atomicMax(&sh->taint[n & 1][c], (static_cast<unsigned long long>(n + 1) << 32) | (0x7fffffffu - static_cast<unsigned>(col0 + r)));
+                *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) = n + 1;
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(b_p_full + 8 * sb);
+    }
+  }
+
+  // ================================ tear-down =====================================
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 15) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the parts of the tiles that were cut, in the order of the line: part 0 in slot 1 of the CTA where the tile begins,
+// part i in slot 0 of the i-th CTA behind it.  One warp per row.
+constexpr int kJoinWarps = 8;
+template <int DT> __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const Args a) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Owner own = a.owners[blockIdx.x];
+  const int lane = threadIdx.x & 31;
+  const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+  if (own.parts == 0 || r >= own.ntok * a.group) return;
+  auto place = [&](int i) { return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kBM + r; };
+  float big = -INFINITY;
+  for (int i = lane; i < own.parts; i += 32) {
+    const float2 ml = a.part_ml[place(i)];
+    if (ml.y != 0.f) big = fmaxf(big, ml.x);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < own.parts; ++i) {
+    const long long pr = place(i);
+    const float2 ml = a.part_ml[pr];
+    const float4 o = reinterpret_cast<const float4 *>(a.part_o + pr * kD)[lane];
+    if (ml.y != 0.f) {   // else the row saw nothing of this part
+      const float w = ex2(ml.x - big);
+      l = fmaf(w, ml.y, l);
+      acc.x = fmaf(w, o.x, acc.x);
+      acc.y = fmaf(w, o.y, acc.y);
+      acc.z = fmaf(w, o.z, acc.z);
+      acc.w = fmaf(w, o.w, acc.w);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t *dst = a.out + static_cast<long long>(own.tok0 + r / a.group) * a.out_t + static_cast<long long>(own.kvh * a.group + r % a.group) * a.out_h;
+  reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+}
+
+int map_3d(CUtensorMap *tm, const void *ptr, const cuuint64_t (&dims)[3], const cuuint64_t (&strides)[2],
+           const cuuint32_t (&box)[3], int dtype) {
+  EncodeTiledFnT enc = tma_encode_fn();
+  NB200_REQUIRE(enc, NB200_ERR_LAUNCH, "attn_paged: cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = enc(tm, dtype == NB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  NB200_REQUIRE(r == CUDA_SUCCESS, NB200_ERR_LAUNCH, "attn_paged: cuTensorMapEncodeTiled failed with code %d", (int)r);
+  return NB200_OK;
+}
+
+template <int DT> int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Args &a, cudaStream_t st) {
+  NB200_CHECK_CUDA(cudaFuncSetAttribute(attn_paged_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  int dev = 0, sms = 0;
+  NB200_CHECK_CUDA(cudaGetDevice(&dev));
+  NB200_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  const int grid = sms < kMaxCtas ? sms : kMaxCtas;
+  attn_paged_kernel<DT><<<dim3(grid), dim3(kThreads), kSmemBytes, st>>>(tq, tk, tv, a);
+  NB200_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid, kBM / kJoinWarps);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DT>, a));
+  return NB200_OK;
 }
 
 }  // namespace
@@ -73,7 +841,7 @@ template <int DT> __global__ void __launch_bounds__(32) attn_paged_kernel(const 
 
 using namespace nb200;
 
-extern "C" size_t nb200_attn_paged_workspace_bytes(void) { return 160 * 2 * 128 * (kD + 2) * sizeof(float) + 160 * 64; }
+extern "C" size_t nb200_attn_paged_workspace_bytes(void) { return kPartO + kPartMl + kMaxCtas * sizeof(Owner); }
 
 extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *v_pages, const int *block_table,
                                 const int *cu_seqlens, const int *seq_lens, void *workspace, void *out,
@@ -90,23 +858,43 @@ extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *
   NB200_REQUIRE(page_size == kPageRows, NB200_ERR_UNSUPPORTED, "%s: page_size = %d, only %d rows per page is implemented", who,
                 page_size, kPageRows);
   NB200_REQUIRE(Hq % Hkv == 0, NB200_ERR_UNSUPPORTED, "%s: Hq %% Hkv != 0", who);
-  NB200_REQUIRE(Hq / Hkv <= 128, NB200_ERR_UNSUPPORTED, "%s: more than 128 query heads per kv head", who);
+  NB200_REQUIRE(Hq / Hkv <= kBM, NB200_ERR_UNSUPPORTED, "%s: more than 128 query heads per kv head", who);
   NB200_REQUIRE(Hq <= 65535, NB200_ERR_UNSUPPORTED, "%s: too many heads", who);
-  NB200_REQUIRE(max_pages <= (0x7fffffff / kPageRows), NB200_ERR_UNSUPPORTED, "%s: max_pages * page_size does not fit 31 bits", who);
-  NB200_REQUIRE(static_cast<long long>(num_pages) * Hkv < (1ll << 31), NB200_ERR_UNSUPPORTED,
+  NB200_REQUIRE(T < (1 << 30) && max_pages <= (1 << 30) / kPageRows, NB200_ERR_UNSUPPORTED,
+                "%s: T or max_pages * page_size does not fit 30 bits", who);
+  NB200_REQUIRE(static_cast<long long>(num_pages) * Hkv < (1ll << 31) - 1, NB200_ERR_UNSUPPORTED,
                 "%s: num_pages * Hkv does not fit 31 bits", who);
   NB200_REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace),
                 NB200_ERR_BAD_ARG, "%s: q, out, the page pools and the workspace must be 16-byte aligned", who);
-  for (int i = 0; i < 4; ++i)
-    NB200_REQUIRE(strides[i] >= 0 && strides[i] % 8 == 0, NB200_ERR_BAD_ARG,
-                  "%s: the strides of q and out must be multiples of 16 bytes", who);
-  Args a{q, k_pages, v_pages, out, block_table, cu_seqlens, seq_lens, strides[0], strides[1], strides[2], strides[3],
-         T, B, Hq, Hkv, num_pages, max_pages, scale_log2, status};
+  const int extents[4] = {T, Hq, T, Hq};
+  long long s[4];
+  for (int i = 0; i < 4; ++i) {
+    s[i] = extents[i] == 1 ? kD : strides[i];              // a stride that is never taken
+    NB200_REQUIRE(s[i] >= kD && s[i] % 8 == 0 && s[i] < (1ll << 38), NB200_ERR_BAD_ARG,
+                  "%s: the strides of q and out must be multiples of 16 bytes, at least a row", who);
+  }
+  Args a{};
+  a.block_table = block_table, a.cu_seqlens = cu_seqlens, a.seq_lens = seq_lens;
+  a.out = static_cast<uint16_t *>(out), a.out_t = s[2], a.out_h = s[3];
+  a.T = T, a.B = B, a.Hkv = Hkv, a.group = Hq / Hkv, a.tok_tile = kBM / a.group;
+  a.num_pages = num_pages, a.max_pages = max_pages, a.scale_log2 = scale_log2, a.status = status;
+  char *ws = static_cast<char *>(workspace);
+  a.part_o = reinterpret_cast<float *>(ws);
+  a.part_ml = reinterpret_cast<float2 *>(ws + kPartO);
+  a.owners = reinterpret_cast<Owner *>(ws + kPartO + kPartMl);
+  CUtensorMap tq, tk, tv;
+  int rc;
+  // rows of a Q tile: tokens, and the group's heads inside a token
+  if ((rc = map_3d(&tq, q, {kD, static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)},
+                   {static_cast<cuuint64_t>(s[1]) * 2, static_cast<cuuint64_t>(s[0]) * 2},
+                   {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(a.tok_tile)}, dtype)) != NB200_OK)
+    return rc;
+  const cuuint64_t slices = static_cast<cuuint64_t>(num_pages) * Hkv;
+  if ((rc = map_3d(&tk, k_pages, {kD, kPageRows, slices}, {kD * 2, kPageRows * kD * 2}, {64, kPageRows, 1}, dtype)) != NB200_OK)
+    return rc;
+  if ((rc = map_3d(&tv, v_pages, {kD, kPageRows, slices}, {kD * 2, kPageRows * kD * 2}, {64, kPageRows, 1}, dtype)) != NB200_OK)
+    return rc;
   auto st = static_cast<cudaStream_t>(stream);
-  if (dtype == NB200_BF16)
-    attn_paged_kernel<NB200_BF16><<<dim3(T, Hq), 32, 0, st>>>(a);
-  else
-    attn_paged_kernel<NB200_F16><<<dim3(T, Hq), 32, 0, st>>>(a);
-  NB200_CHECK_CUDA(cudaGetLastError());
-  return NB200_OK;
+  if (dtype == NB200_BF16) return launch<NB200_BF16>(tq, tk, tv, a, st);
+  return launch<NB200_F16>(tq, tk, tv, a, st);
 }

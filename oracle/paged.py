@@ -40,7 +40,7 @@ def attn_paged(q, k_pages, v_pages, table, cu, lens, scale: float):
     T, Hq, D = q.shape
     Hkv = k_pages.shape[1]
     group = Hq // Hkv
-    out = torch.full((T, Hq, D), float("nan"), dtype=torch.float64)
+    out = torch.full((T, Hq, D), float("nan"), dtype=torch.float64, device=q.device)
     spread, score = torch.zeros_like(out), 0.0
     for b, length in enumerate(lens):
         n = cu[b + 1] - cu[b]
@@ -50,8 +50,8 @@ def attn_paged(q, k_pages, v_pages, table, cu, lens, scale: float):
         pages = table[b, :(used + PAGE - 1) // PAGE].long()
         k = k_pages[pages].transpose(1, 2).reshape(-1, Hkv, D)[:used].double()
         v = v_pages[pages].transpose(1, 2).reshape(-1, Hkv, D)[:used].double()
-        pos = length - n + torch.arange(n)
-        sees = torch.arange(used)[None] <= pos[:, None]
+        pos = length - n + torch.arange(n, device=q.device)
+        sees = torch.arange(used, device=q.device)[None] <= pos[:, None]
         for h in range(Hq):
             qh, kh, vh = q[cu[b]:cu[b + 1], h].double(), k[:, h // group], v[:, h // group]
             x = (qh @ kh.T * scale).masked_fill(~sees, float("-inf"))

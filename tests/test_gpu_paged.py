@@ -353,6 +353,39 @@ def test_chunk_attention_with_strided_queries_and_output(cuda, native_lib):
     assert bool((wide[..., :D] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=NAMES.get)
+def test_chunk_attention_keeps_non_finite_rows_to_those_that_see_them(cuda, native_lib, dtype):
+    """A value of one new token is infinite, another's is NaN, a key of a third is NaN: rows before them are as if they
+    were not there, rows that see them are not finite in that column (value) or at all (key)."""
+    new, lens = [150, 4], [700, 300]
+    batch = Batch(new, lens, 2, dtype)
+    q = randn((batch.T, 8, D), 31, dtype)
+
+    def place(b, j):
+        return batch.table[b, j // PAGE].long(), j % PAGE
+
+    page, row = place(0, 550 + 37)
+    batch.v[page, 0, row, 77] = float("inf")
+    page, row = place(0, 550 + 90)
+    batch.v[page, 1, row, 3] = float("nan")
+    page, row = place(1, 298)
+    batch.k[page, 1, row, 5] = float("nan")
+    out = attend(batch, q.to(cuda), cuda).cpu()
+    finish()
+    hidden = [(0, 77, range(37)), (1, 3, range(90))]
+    batch.k = batch.k.nan_to_num(0.0)
+    batch.v = batch.v.nan_to_num(0.0, posinf=0.0)
+    exact, spread, score = paged.attn_paged(q, batch.k, batch.v, batch.table, batch.cu, batch.lens, 1 / math.sqrt(D))
+    for h, col, _ in hidden:
+        seen = out[:150, 4 * h:4 * h + 4, col]
+        assert bool(seen[(37, 90)[h]:].isfinite().logical_not().all()) and bool(seen[:(37, 90)[h]].isfinite().all())
+        rows = slice((37, 90)[h], 150)
+        out[rows, 4 * h:4 * h + 4, col] = exact[rows, 4 * h:4 * h + 4, col].to(dtype)
+    assert bool(out[152:154, 4:].isnan().all())
+    out[152:154, 4:] = exact[152:154, 4:].to(dtype)
+    close_to_attention(out[:154], exact[:154], spread[:154], score, 700, 6.0, dtype)
+
+
 def test_chunk_attention_refuses_a_table_entry_outside_the_pool(cuda, native_lib):
     from neptune_mlir import runtime
 
@@ -403,6 +436,27 @@ def test_chunk_attention_with_offsets_beyond_31_bits(cuda, native_lib):
     finish()
     batch.k, batch.v = big_k[-batch.num_pages:].cpu(), big_v[-batch.num_pages:].cpu()
     check_attention(batch, q_out.cpu(), out)
+
+
+@pytest.mark.parametrize("dtype,Hq,Hkv,new,lens", [
+    (torch.bfloat16, 40, 8, [(5 * i) % 8 for i in range(32)], [1 + (1237 * i) % 16001 for i in range(32)]),
+    (torch.float16, 32, 8, [499] + [1] * 15, [4299] + [1 + (1811 * i) % 7600 for i in range(15)]),
+    (torch.bfloat16, 16, 1, [300, 200, 5, 1], [6000, 200, 20000, 333]),
+], ids=["drafts", "mixed", "wide"])
+def test_chunk_attention_streams_many_long_sequences(cuda, native_lib, dtype, Hq, Hkv, new, lens):
+    """A cache larger than the L2: blocks arrive late and in bursts, while every CTA goes through parts of many tiles.
+    The definition in 64 bits is evaluated on the device."""
+    lens = [max(n, length) for n, length in zip(new, lens)]
+    batch = Batch(new, lens, Hkv, dtype)
+    q = randn((batch.T, Hq, D), 32, dtype).to(cuda)
+    batch.k, batch.v, batch.table = batch.k.to(cuda), batch.v.to(cuda), batch.table.to(cuda)
+    exact, spread, score = paged.attn_paged(q, batch.k, batch.v, batch.table, batch.cu, lens, 1 / math.sqrt(D))
+    total, vmax = batch.cu[-1], batch.v.nan_to_num(0.0).abs().max().item()
+    for _ in range(3):
+        out = attend(batch, q, cuda)
+        close_to_attention(out[:total], exact[:total].cpu(), spread[:total].cpu(), score, max(lens), vmax, dtype)
+        assert bool((out[total:].float() == 7.0).all())
+    finish()
 
 
 def test_chunk_attention_is_the_same_twice(cuda, native_lib):

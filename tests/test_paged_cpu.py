@@ -69,8 +69,9 @@ def test_attn_paged_rejects_bad_calls_without_a_gpu(native_lib, ptr):
             (dict(work=None), -1, b"null pointer"), (dict(T=0), -1, b"non-positive"), (dict(scale=0.0), -1, b"scale_log2"),
             (dict(scale=math.nan), -1, b"scale_log2"), (dict(dtype=2), -2, b"f16 and bf16 only"), (dict(D=64), -2, b"only 128"),
             (dict(page=32), -2, b"only 64 rows per page"), (dict(Hq=7), -2, b"Hq % Hkv"), (dict(Hq=258), -2, b"128 query heads"),
-            (dict(q=p + 8), -1, b"16-byte aligned"), (dict(strides=longs(1020, 128, 1024, 128)), -1, b"strides"),
-            (dict(strides=longs(-1024, 128, 1024, 128)), -1, b"strides"), (dict(max_pages=1 << 25), -2, b"31 bits"),
+            (dict(q=p + 8), -1, b"16-byte aligned"), (dict(T=2, strides=longs(1020, 128, 1024, 128)), -1, b"strides"),
+            (dict(T=2, strides=longs(-1024, 128, 1024, 128)), -1, b"strides"), (dict(strides=longs(1024, 128, 1024, 0)), -1, b"strides"),
+            (dict(T=1 << 30), -2, b"30 bits"), (dict(max_pages=1 << 25), -2, b"30 bits"),
             (dict(pages=1 << 30), -2, b"num_pages * Hkv")):
         assert call(**kwargs) == code and text in lib.nb200_last_error(), kwargs
 
