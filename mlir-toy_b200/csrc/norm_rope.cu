@@ -9,15 +9,19 @@
 // once, on the way out.  The angle is reduced to a fraction of a turn in fp64: p * f in fp32 would be off by 0.06 rad at
 // position 10^6.
 //
-// One CTA per token (and, for few tokens, per group of its rows): a row is read by G lanes, 8 elements each, so a thread
-// holds U rows at once and its loads are in flight while 64 threads compute the token's sines and cosines.  A pair's
-// other half is eight shuffles away; a row is read and written once, so the call is bound by HBM.
+// A warp takes a token, or part of its rows where there are few tokens.  A row is read by G lanes, and lane u holds the
+// elements {4u .. 4u+3} and {rot/2 + 4u ..} (halves) or {8u .. 8u+7} (neighbours): both elements of a pair and the same
+// four angles either way, so a rotation needs no shuffle, and the sines and cosines, which a lane computes two of, are
+// read from shared memory once for all the rows of the token.  No barrier wider than a warp; four rows' loads are in
+// flight at a time.
 #include "nb200_common.cuh"
 
 namespace nb200 {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;             // rows of a lane in flight
 constexpr int kMaxHalf = 128;          // rot <= 256
 constexpr int kPageRows = 64;
 constexpr int kCacheD = 128;
@@ -44,49 +48,33 @@ struct Args {
   int *status;
 };
 
-// Eight consecutive elements of a row as they are stored.
-template <int DT> struct Raw {
-  uint4 w[DT == NB200_F32 ? 2 : 1];
+// Four consecutive elements of a row as they are stored: 8 bytes, or 16 in fp32.
+template <int DT> struct Piece {
+  using type = uint2;
 };
-template <int DT> __device__ __forceinline__ Raw<DT> load_raw(const void *base, long long elem) {
-  Raw<DT> r;
-  const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(base) + elem * (DT == NB200_F32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < (DT == NB200_F32 ? 2 : 1); ++i) r.w[i] = p[i];
-  return r;
+template <> struct Piece<NB200_F32> {
+  using type = uint4;
+};
+template <int DT> using piece_t = typename Piece<DT>::type;
+template <int DT> __device__ __forceinline__ piece_t<DT> load_piece(const void *base, long long elem) {
+  return *reinterpret_cast<const piece_t<DT> *>(static_cast<const char *>(base) + elem * (DT == NB200_F32 ? 4 : 2));
 }
-template <int DT> __device__ __forceinline__ void store_raw(void *base, long long elem, const Raw<DT> &r) {
-  uint4 *p = reinterpret_cast<uint4 *>(static_cast<char *>(base) + elem * (DT == NB200_F32 ? 4 : 2));
-#pragma unroll
-  for (int i = 0; i < (DT == NB200_F32 ? 2 : 1); ++i) p[i] = r.w[i];
+template <int DT> __device__ __forceinline__ void store_piece(void *base, long long elem, piece_t<DT> x) {
+  *reinterpret_cast<piece_t<DT> *>(static_cast<char *>(base) + elem * (DT == NB200_F32 ? 4 : 2)) = x;
 }
-template <int DT> __device__ __forceinline__ void to_float(const Raw<DT> &r, float (&y)[8]) {
-  const uint32_t *w = reinterpret_cast<const uint32_t *>(&r);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (DT == NB200_F32) {
-      y[2 * i] = __uint_as_float(w[2 * i]);
-      y[2 * i + 1] = __uint_as_float(w[2 * i + 1]);
-    } else {
-      const float2 f = unpack2<DT>(w[i]);
-      y[2 * i] = f.x;
-      y[2 * i + 1] = f.y;
-    }
+template <int DT> __device__ __forceinline__ void to_float(piece_t<DT> r, float *y) {
+  if constexpr (DT == NB200_F32) {
+    y[0] = __uint_as_float(r.x), y[1] = __uint_as_float(r.y), y[2] = __uint_as_float(r.z), y[3] = __uint_as_float(r.w);
+  } else {
+    const float2 f = unpack2<DT>(r.x), g = unpack2<DT>(r.y);
+    y[0] = f.x, y[1] = f.y, y[2] = g.x, y[3] = g.y;
   }
 }
-template <int DT> __device__ __forceinline__ Raw<DT> from_float(const float (&y)[8]) {
-  Raw<DT> r;
-  uint32_t *w = reinterpret_cast<uint32_t *>(&r);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (DT == NB200_F32) {
-      w[2 * i] = __float_as_uint(y[2 * i]);
-      w[2 * i + 1] = __float_as_uint(y[2 * i + 1]);
-    } else {
-      w[i] = pack2<DT>(y[2 * i], y[2 * i + 1]);
-    }
-  }
-  return r;
+template <int DT> __device__ __forceinline__ piece_t<DT> from_float(const float *y) {
+  if constexpr (DT == NB200_F32)
+    return make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+  else
+    return make_uint2(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]));
 }
 
 __device__ __forceinline__ void report(int *status, int code, int detail, int detail2) {
@@ -97,54 +85,55 @@ __device__ __forceinline__ void report(int *status, int code, int detail, int de
   }
 }
 
-// Rows of a token: Hq queries, then Hkv keys, then (append) Hkv values.
-template <int DT, int G, int U, bool APPEND>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a) {
-  constexpr int kRows = kThreads / G;
-  __shared__ float2 turn[kMaxHalf];                       // (cos, sin) of the token's angles
-  const long long t = blockIdx.x;
-  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-  const int row0 = blockIdx.y * (kRows * U) + sub;
-  const int rows = a.Hq + (APPEND ? 2 : 1) * a.Hkv;
-  const int c0 = lane * 8;
-  const bool in_row = c0 < a.D;
-  const long long bt = APPEND ? 0 : t / a.S, st = APPEND ? t : t % a.S;
-
-  Raw<DT> raw[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int row = row0 + u * kRows;
-    raw[u] = Raw<DT>{};
-    if (in_row && row < rows) {
-      if (row < a.Hq)
-        raw[u] = load_raw<DT>(a.q, bt * a.sq.b + st * a.sq.t + row * a.sq.h + c0);
-      else if (!APPEND || row < a.Hq + a.Hkv)
-        raw[u] = load_raw<DT>(a.k, bt * a.sk.b + st * a.sk.t + (row - a.Hq) * a.sk.h + c0);
-      else
-        raw[u] = load_raw<DT>(a.v, st * a.sv.t + (row - a.Hq - a.Hkv) * a.sv.h + c0);
-    }
+// Sequence whose tokens include row t, or -1: one before the first entry of cu_seqlens [B + 1] above t, found 32 ways at
+// a time by the whole warp.
+__device__ __forceinline__ int sequence_of(const int *cu, int B, int t, int lane) {
+  int lo = 0, n = B + 1;                                  // entries [0, lo) are <= t; the first above t is in [lo, lo + n]
+  while (n > 0) {
+    const int step = (n + 31) / 32, i = lo + lane * step;
+    const int below = __popc(__ballot_sync(0xffffffffu, lane * step < n && cu[min(i, B)] <= t));
+    if (below == 0) break;                                // entry lo is above t
+    const int probe = lo + (below - 1) * step;            // the last probe that is <= t
+    n = min(step - 1, lo + n - probe - 1);
+    lo = probe + 1;
   }
+  return lo - 1 < B ? lo - 1 : -1;
+}
+
+// Rows of a token: Hq queries, then Hkv keys, then (append) Hkv values.  Warp `unit` of the grid takes the passes
+// [chunk * per, chunk * per + per) of a token, 32 / G rows each.
+template <int DT, int G, bool APPEND>
+__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a, const long long units, const int chunks, const int per) {
+  constexpr int kRows = 32 / G;
+  __shared__ float4 turns[kWarps][kMaxHalf / 2];          // (cos, sin) of the token's angles, two to a word
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  if (unit >= units) return;
+  const int t = static_cast<int>(unit / chunks), chunk = static_cast<int>(unit % chunks);
+  const int u = lane % G, sub = lane / G;
+  const int rows = a.Hq + (APPEND ? 2 : 1) * a.Hkv;
+  const bool in_row = u * 8 < a.D;
+  const bool turned = u * 8 < a.rot;
+  // first elements of the lane's two pieces
+  const int e0 = turned && !a.interleaved ? 4 * u : 8 * u, e1 = turned && !a.interleaved ? a.rot / 2 + 4 * u : 8 * u + 4;
+  const long long bt = APPEND ? 0 : t / a.S, st = APPEND ? t : t % a.S;
 
   int pos = 0;
   long long slot_base = 0;                                // element offset of (page, head 0, row) in the pools
   if constexpr (APPEND) {
-    // the sequence whose tokens include t: one past the last entry of cu_seqlens that is <= t
-    int below = 0;
-    for (int i = 0; i <= a.B; i += kThreads)
-      below += __syncthreads_count(i + static_cast<int>(threadIdx.x) <= a.B && a.cu_seqlens[min(i + static_cast<int>(threadIdx.x), a.B)] <= t);
-    const int b = below - 1;
-    if (b < 0 || b >= a.B) return;                        // a row behind the last sequence: left as it was
+    const int b = sequence_of(a.cu_seqlens, a.B, t, lane);
+    if (b < 0) return;                                    // a row of no sequence: left as it was
     const int first = a.cu_seqlens[b], end = a.cu_seqlens[b + 1];
     if (t < first || t >= end) return;                    // cu_seqlens is not a running sum
     const long long p = static_cast<long long>(a.seq_lens[b]) - end + t;
     if (p < 0 || p >= static_cast<long long>(a.max_pages) * kPageRows) {
-      if (threadIdx.x == 0 && blockIdx.y == 0) report(a.status, kErrSlot, static_cast<int>(t), static_cast<int>(p));
+      if (lane == 0 && chunk == 0) report(a.status, kErrSlot, t, static_cast<int>(p));
       return;
     }
     pos = static_cast<int>(p);
     const int page = a.block_table[static_cast<long long>(b) * a.max_pages + pos / kPageRows];
     if (page < 0 || page >= a.num_pages) {
-      if (threadIdx.x == 0 && blockIdx.y == 0) report(a.status, kErrTable, page, static_cast<int>(threadIdx.x));
+      if (lane == 0 && chunk == 0) report(a.status, kErrTable, page, 0);
       return;
     }
     slot_base = (static_cast<long long>(page) * a.Hkv * kPageRows + pos % kPageRows) * kCacheD;
@@ -152,87 +141,110 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a) {
     pos = a.positions[bt * a.positions_b + st];
   }
 
-  for (int i = threadIdx.x; i < a.rot / 2; i += kThreads) {
-    const double turns = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;   // 1 / 2 pi
-    float s, c;
-    sincospif(2.f * static_cast<float>(turns - rint(turns)), &s, &c);
-    turn[i] = make_float2(c, s);
-  }
-  __syncthreads();
+  const void *const q = static_cast<const char *>(a.q) + (bt * a.sq.b + st * a.sq.t) * (DT == NB200_F32 ? 4 : 2);
+  const void *const k = static_cast<const char *>(a.k) + (bt * a.sk.b + st * a.sk.t) * (DT == NB200_F32 ? 4 : 2);
+  const void *const v = APPEND ? static_cast<const char *>(a.v) + st * a.sv.t * 2 : nullptr;
 
+  for (int i = lane; i < a.rot / 2; i += 32) {
+    const double x = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;   // 1 / 2 pi
+    float s, c;
+    sincospif(2.f * static_cast<float>(x - rint(x)), &s, &c);
+    reinterpret_cast<float2 *>(turns[warp])[i] = make_float2(c, s);
+  }
+  __syncwarp();
+  float4 cs[2] = {};                                      // of the angles 4u .. 4u + 3
+  if (turned) cs[0] = turns[warp][2 * u], cs[1] = turns[warp][2 * u + 1];
+  piece_t<DT> wq0{}, wq1{}, wk0{}, wk1{};
+  if (in_row && a.wq) wq0 = load_piece<DT>(a.wq, e0), wq1 = load_piece<DT>(a.wq, e1);
+  if (in_row && a.wk) wk0 = load_piece<DT>(a.wk, e0), wk1 = load_piece<DT>(a.wk, e1);
+
+  const int first_row = chunk * per * kRows + sub, last_row = min(rows, (chunk + 1) * per * kRows);
+  for (int row0 = first_row; row0 - sub < last_row; row0 += kUnroll * kRows) {
+    piece_t<DT> x0[kUnroll], x1[kUnroll];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int row = row0 + u * kRows;
-    const bool is_q = row < a.Hq, is_v = APPEND && row >= a.Hq + a.Hkv;
-    const void *w = is_q ? a.wq : a.wk;
-    float y[8];
-    to_float<DT>(raw[u], y);
-    if (a.wq || a.wk) {                                   // uniform: every lane takes part in the sum
-      float ss = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (w && in_row) {
-        const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
-        float g[8];
-        to_float<DT>(load_raw<DT>(w, c0), g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] * r * g[i];
+    for (int i = 0; i < kUnroll; ++i) {
+      const int row = row0 + i * kRows;
+      x0[i] = x1[i] = piece_t<DT>{};
+      if (in_row && row < last_row) {
+        const void *src = q;
+        long long at = row * a.sq.h;
+        if (row >= a.Hq) src = k, at = (row - a.Hq) * a.sk.h;
+        if (APPEND && row >= a.Hq + a.Hkv) src = v, at = (row - a.Hq - a.Hkv) * a.sv.h;
+        x0[i] = load_piece<DT>(src, at + e0);
+        x1[i] = load_piece<DT>(src, at + e1);
       }
     }
-    if (a.interleaved) {
-      if (c0 < a.rot) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 cs = turn[c0 / 2 + i];
-          const float y1 = y[2 * i], y2 = y[2 * i + 1];
-          y[2 * i] = y1 * cs.x - y2 * cs.y;
-          y[2 * i + 1] = y2 * cs.x + y1 * cs.y;
+    for (int i = 0; i < kUnroll; ++i) {
+      const int row = row0 + i * kRows;
+      if (row - sub >= last_row) break;                   // the same for the whole warp
+      const bool is_q = row < a.Hq, is_v = APPEND && row >= a.Hq + a.Hkv;
+      float y[8];
+      to_float<DT>(x0[i], y);
+      to_float<DT>(x1[i], y + 4);
+      if (a.wq || a.wk) {                                 // every lane takes part in the sum
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (is_q ? a.wq != nullptr : a.wk != nullptr) {
+          const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
+          float g[8];
+          to_float<DT>(is_q ? wq0 : wk0, g);
+          to_float<DT>(is_q ? wq1 : wk1, g + 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = y[e] * r * g[e];
         }
       }
-    } else {
-      // the other half of the pairs of this lane's 8 elements sits rot / 16 lanes up or down
-      const int half = a.rot / 16;
-      const bool low = lane < half;
-      const int other = low ? lane + half : (lane < 2 * half ? lane - half : lane);
-      float z[8];
+      if (turned) {
+        const float c[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, s[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
+        if (a.interleaved) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) z[i] = __shfl_sync(0xffffffffu, y[i], other, G);
-      if (lane < 2 * half) {
-        const int i0 = (low ? lane : lane - half) * 8;
+          for (int e = 0; e < 4; ++e) {
+            const float y1 = y[2 * e], y2 = y[2 * e + 1];
+            y[2 * e] = y1 * c[e] - y2 * s[e];
+            y[2 * e + 1] = y2 * c[e] + y1 * s[e];
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 cs = turn[i0 + i];
-          y[i] = fmaf(low ? -z[i] : z[i], cs.y, y[i] * cs.x);
+          for (int e = 0; e < 4; ++e) {
+            const float y1 = y[e], y2 = y[e + 4];
+            y[e] = y1 * c[e] - y2 * s[e];
+            y[e + 4] = y2 * c[e] + y1 * s[e];
+          }
         }
       }
-    }
-    if (in_row && row < rows) {
-      if (is_q)
-        store_raw<DT>(a.q_out, bt * a.sqo.b + st * a.sqo.t + row * a.sqo.h + c0, from_float<DT>(y));
-      else if constexpr (!APPEND)
-        store_raw<DT>(a.k_out, bt * a.sko.b + st * a.sko.t + (row - a.Hq) * a.sko.h + c0, from_float<DT>(y));
-      else if (is_v)
-        store_raw<DT>(a.v_pages, slot_base + static_cast<long long>(row - a.Hq - a.Hkv) * (kPageRows * kCacheD) + c0, raw[u]);
-      else
-        store_raw<DT>(a.k_pages, slot_base + static_cast<long long>(row - a.Hq) * (kPageRows * kCacheD) + c0, from_float<DT>(y));
+      if (in_row && row < last_row) {
+        void *dst = a.q_out;
+        long long at = bt * a.sqo.b + st * a.sqo.t + row * a.sqo.h;
+        if constexpr (APPEND) {
+          if (!is_q) dst = a.k_pages, at = slot_base + static_cast<long long>(row - a.Hq) * (kPageRows * kCacheD);
+          if (is_v) dst = a.v_pages, at = slot_base + static_cast<long long>(row - a.Hq - a.Hkv) * (kPageRows * kCacheD);
+        } else {
+          if (!is_q) dst = a.k_out, at = bt * a.sko.b + st * a.sko.t + (row - a.Hq) * a.sko.h;
+        }
+        store_piece<DT>(dst, at + e0, is_v ? x0[i] : from_float<DT>(y));
+        store_piece<DT>(dst, at + e1, is_v ? x1[i] : from_float<DT>(y + 4));
+      }
     }
   }
 }
 
-template <int DT, int G, int U, bool APPEND> int launch_u(const Args &a, long long tokens, int rows, cudaStream_t st) {
-  const int per = kThreads / G * U;
-  norm_rope_kernel<DT, G, U, APPEND><<<dim3(static_cast<unsigned>(tokens), static_cast<unsigned>((rows + per - 1) / per)), kThreads, 0, st>>>(a);
+// A warp does all the rows of a token where the tokens alone fill the SMs' warps; with fewer tokens their rows are dealt
+// out, down to one pass per warp, which then computes the token's angles again.
+template <int DT, int G, bool APPEND> int launch_g(const Args &a, long long tokens, int rows, cudaStream_t st) {
+  constexpr int kResident = 148 * 32;
+  const int passes = (rows + 32 / G - 1) / (32 / G);
+  long long per = tokens * passes / kResident;
+  per = per < 1 ? 1 : (per >= passes ? passes : per);
+  if (per > kUnroll) per = (per + kUnroll - 1) / kUnroll * kUnroll;
+  const int chunks = static_cast<int>((passes + per - 1) / per);
+  const long long units = tokens * chunks, blocks = (units + kWarps - 1) / kWarps;
+  NB200_REQUIRE(blocks < (1ll << 31), NB200_ERR_UNSUPPORTED, "norm and rotation: too many rows");
+  norm_rope_kernel<DT, G, APPEND><<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, st>>>(a, units, chunks, static_cast<int>(per));
   NB200_CHECK_CUDA(cudaGetLastError());
   return NB200_OK;
-}
-template <int DT, int G, bool APPEND> int launch_g(const Args &a, long long tokens, int rows, cudaStream_t st) {
-  const int passes = (rows + kThreads / G - 1) / (kThreads / G);
-  if (passes == 1 || tokens * passes <= 4 * 148) return launch_u<DT, G, 1, APPEND>(a, tokens, rows, st);
-  if (passes == 2) return launch_u<DT, G, 2, APPEND>(a, tokens, rows, st);
-  if (passes == 3) return launch_u<DT, G, 3, APPEND>(a, tokens, rows, st);
-  return launch_u<DT, G, 4, APPEND>(a, tokens, rows, st);
 }
 template <int DT> int launch_dense(const Args &a, long long tokens, cudaStream_t st) {
   const int rows = a.Hq + a.Hkv;
