@@ -27,6 +27,8 @@ OBJ_DIR = PKG / "build"
 OUT = PKG / "neptune_mlir" / "_native" / "libnb200.so"
 FRONT_SRC = CSRC / "htile_front" / "htile_front.cpp"
 FRONT_OUT = PKG / "neptune_mlir" / "_native" / "libhtile_front.so"
+BINDING_SRC = CSRC / "torch_binding" / "torch_binding.cpp"
+BINDING_OUT = PKG / "neptune_mlir" / "_native" / "nb200_torch.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -61,6 +63,13 @@ def _compile(src: Path, obj: Path, verbose: bool) -> str:
     return log
 
 
+def _compile_all(jobs, verbose: bool) -> None:
+    if jobs:
+        with concurrent.futures.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
+            for fut in [ex.submit(_compile, s, o, verbose) for s, o in jobs]:
+                fut.result()
+
+
 def build_front(force: bool = False) -> Path:
     """The HTile front end: host C++ only (g++), a shared library of its own next to the kernel library."""
     FRONT_OUT.parent.mkdir(parents=True, exist_ok=True)
@@ -77,6 +86,31 @@ def build_front(force: bool = False) -> Path:
     return FRONT_OUT
 
 
+def build_binding(force: bool = False) -> Path:
+    """The CPython module that calls the kernel library with torch tensors: g++ against torch's headers and libraries."""
+    BINDING_OUT.parent.mkdir(parents=True, exist_ok=True)
+    newest = max(BINDING_SRC.stat().st_mtime, (INCLUDE / "nb200.h").stat().st_mtime)
+    if force or not BINDING_OUT.exists() or BINDING_OUT.stat().st_mtime < newest:
+        import sysconfig
+
+        import torch
+
+        gxx = shutil.which("g++") or shutil.which("c++")
+        if gxx is None:
+            raise RuntimeError("g++ not found; the torch binding cannot be built")
+        root = Path(torch.__file__).resolve().parent
+        cuda = Path(_nvcc()).resolve().parents[1]
+        cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               f"-I{INCLUDE}", f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+               f"-isystem{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(BINDING_OUT),
+               f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-Wl,--unresolved-symbols=ignore-all",
+               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+    return BINDING_OUT
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(exist_ok=True)
     OUT.parent.mkdir(parents=True, exist_ok=True)
@@ -89,10 +123,10 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         stale = force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, hdr_time)
         if stale:
             jobs.append((src, obj))
-    if jobs:
-        with concurrent.futures.ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 4)) as ex:
-            for fut in [ex.submit(_compile, s, o, verbose) for s, o in jobs]:
-                fut.result()
+    with concurrent.futures.ThreadPoolExecutor(max_workers=1) as other:
+        binding = other.submit(build_binding, force)
+        _compile_all(jobs, verbose)
+        binding.result()
     objs = [OBJ_DIR / (s.stem + ".o") for s in sources]
     if jobs or not OUT.exists() or any(o.stat().st_mtime > OUT.stat().st_mtime for o in objs):
         cmd = [_nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static",

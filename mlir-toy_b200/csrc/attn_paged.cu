@@ -37,6 +37,8 @@
 // Every wait is bounded; on expiry the CTA records a code in the status words and unwinds.
 #include <cuda.h>
 
+#include <atomic>
+
 #include "nb200_common.cuh"
 #include "sm100_primitives.cuh"
 #include "tma_host.cuh"
@@ -815,16 +817,27 @@ int map_3d(CUtensorMap *tm, const void *ptr, const cuuint64_t (&dims)[3], const 
   return NB200_OK;
 }
 
-template <int DT> int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Args &a, cudaStream_t st) {
-  NB200_CHECK_CUDA(cudaFuncSetAttribute(attn_paged_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
-  int dev = 0, sms = 0;
+// Multiprocessors of the current device, looked up once per device together with the kernel's shared-memory limit.
+template <int DT> int device_sms(int *sms) {
+  static std::atomic<int> known[64];
+  int dev = 0;
   NB200_CHECK_CUDA(cudaGetDevice(&dev));
-  NB200_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64 && (*sms = known[dev].load(std::memory_order_acquire)) > 0) return NB200_OK;
+  NB200_CHECK_CUDA(cudaFuncSetAttribute(attn_paged_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  NB200_CHECK_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev].store(*sms, std::memory_order_release);
+  return NB200_OK;
+}
+
+template <int DT> int launch(const CUtensorMap &tq, const CUtensorMap &tk, const CUtensorMap &tv, const Args &a, cudaStream_t st) {
+  int sms = 0, rc;
+  if ((rc = device_sms<DT>(&sms)) != NB200_OK) return rc;
   const int grid = sms < kMaxCtas ? sms : kMaxCtas;
   attn_paged_kernel<DT><<<dim3(grid), dim3(kThreads), kSmemBytes, st>>>(tq, tk, tv, a);
   NB200_CHECK_CUDA(cudaGetLastError());
+  const int rows = a.T < a.tok_tile ? a.T * a.group : a.tok_tile * a.group;   // of the fullest tile
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, kBM / kJoinWarps);
+  cfg.gridDim = dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps);
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = st;
   cudaLaunchAttribute attr{};

@@ -100,22 +100,25 @@ __device__ __forceinline__ int sequence_of(const int *cu, int B, int t, int lane
   return lo - 1 < B ? lo - 1 : -1;
 }
 
-// Rows of a token: Hq queries, then Hkv keys, then (append) Hkv values.  Warp `unit` of the grid takes the passes
-// [chunk * per, chunk * per + per) of a token, 32 / G rows each.
-template <int DT, int G, bool APPEND>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a, const long long units, const int chunks, const int per) {
+// Rows of a token: Hq queries, then Hkv keys, then (append) Hkv values.  Warp `unit` of the grid takes rows
+// [chunk * per, chunk * per + per) of a token, 32 / G at a time.
+//
+// What bounds it beside HBM is the issue rate, so the arithmetic is on packed pairs of fp32, the weights are converted
+// once per token, and pointers advance by adding: 184 warp instructions per 32 / G rows went down to about 70.
+template <int DT, int G, bool APPEND, bool NEIGHBOURS>
+__global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, const unsigned units, const unsigned chunks, const int per) {
   constexpr int kRows = 32 / G;
+  constexpr int kSize = DT == NB200_F32 ? 4 : 2;
   __shared__ float4 turns[kWarps][kMaxHalf / 2];          // (cos, sin) of the token's angles, two to a word
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + warp;
+  const unsigned unit = blockIdx.x * kWarps + warp;
   if (unit >= units) return;
   const int t = static_cast<int>(unit / chunks), chunk = static_cast<int>(unit % chunks);
   const int u = lane % G, sub = lane / G;
-  const int rows = a.Hq + (APPEND ? 2 : 1) * a.Hkv;
   const bool in_row = u * 8 < a.D;
   const bool turned = u * 8 < a.rot;
-  // first elements of the lane's two pieces
-  const int e0 = turned && !a.interleaved ? 4 * u : 8 * u, e1 = turned && !a.interleaved ? a.rot / 2 + 4 * u : 8 * u + 4;
+  // byte offsets of the lane's two pieces
+  const int e0 = (turned && !NEIGHBOURS ? 4 * u : 8 * u) * kSize, e1 = (turned && !NEIGHBOURS ? a.rot / 2 + 4 * u : 8 * u + 4) * kSize;
   const long long bt = APPEND ? 0 : t / a.S, st = APPEND ? t : t % a.S;
 
   int pos = 0;
@@ -141,92 +144,123 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a, const
     pos = a.positions[bt * a.positions_b + st];
   }
 
-  const void *const q = static_cast<const char *>(a.q) + (bt * a.sq.b + st * a.sq.t) * (DT == NB200_F32 ? 4 : 2);
-  const void *const k = static_cast<const char *>(a.k) + (bt * a.sk.b + st * a.sk.t) * (DT == NB200_F32 ? 4 : 2);
-  const void *const v = APPEND ? static_cast<const char *>(a.v) + st * a.sv.t * 2 : nullptr;
-
-  for (int i = lane; i < a.rot / 2; i += 32) {
-    const double x = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;   // 1 / 2 pi
-    float s, c;
-    sincospif(2.f * static_cast<float>(x - rint(x)), &s, &c);
-    reinterpret_cast<float2 *>(turns[warp])[i] = make_float2(c, s);
+  const int row_lo = chunk * per, row_hi = row_lo + per;
+  if (row_lo < a.Hq + a.Hkv) {                            // else values alone
+    for (int i = lane; i < a.rot / 2; i += 32) {
+      const double x = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;   // 1 / 2 pi
+      float s, c;
+      sincospif(2.f * static_cast<float>(x - rint(x)), &s, &c);
+      reinterpret_cast<float2 *>(turns[warp])[i] = make_float2(c, s);
+    }
   }
   __syncwarp();
-  float4 cs[2] = {};                                      // of the angles 4u .. 4u + 3
-  if (turned) cs[0] = turns[warp][2 * u], cs[1] = turns[warp][2 * u + 1];
-  piece_t<DT> wq0{}, wq1{}, wk0{}, wk1{};
-  if (in_row && a.wq) wq0 = load_piece<DT>(a.wq, e0), wq1 = load_piece<DT>(a.wq, e1);
-  if (in_row && a.wk) wk0 = load_piece<DT>(a.wk, e0), wk1 = load_piece<DT>(a.wk, e1);
+  // cos, sin and -sin of the angles 4u .. 4u + 3, in pairs
+  uint64_t c2[2], s2[2], n2[2];
+  {
+    float4 x = make_float4(1.f, 0.f, 1.f, 0.f), y = x;
+    if (turned) x = turns[warp][2 * u], y = turns[warp][2 * u + 1];
+    c2[0] = f2_pack(x.x, x.z), s2[0] = f2_pack(x.y, x.w), n2[0] = f2_pack(-x.y, -x.w);
+    c2[1] = f2_pack(y.x, y.z), s2[1] = f2_pack(y.y, y.w), n2[1] = f2_pack(-y.y, -y.w);
+  }
 
-  const int first_row = chunk * per * kRows + sub, last_row = min(rows, (chunk + 1) * per * kRows);
-  for (int row0 = first_row; row0 - sub < last_row; row0 += kUnroll * kRows) {
-    piece_t<DT> x0[kUnroll], x1[kUnroll];
+  // queries, then keys
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const int begin = kind ? a.Hq : 0, end = kind ? a.Hq + a.Hkv : a.Hq;
+    const int lo = max(row_lo, begin), hi = min(row_hi, end);
+    if (lo >= hi) continue;
+    const Strides in = kind ? a.sk : a.sq;
+    const char *src = static_cast<const char *>(kind ? a.k : a.q) + (bt * in.b + st * in.t + (lo - begin + sub) * in.h) * kSize + e0;
+    const long long src_step = in.h * kRows * kSize;
+    char *dst;
+    long long dst_step;
+    if (APPEND && kind) {
+      dst = static_cast<char *>(a.k_pages) + (slot_base + static_cast<long long>(lo - begin + sub) * (kPageRows * kCacheD)) * kSize + e0;
+      dst_step = static_cast<long long>(kPageRows) * kCacheD * kRows * kSize;
+    } else {
+      const Strides to = kind ? a.sko : a.sqo;
+      dst = static_cast<char *>(kind ? a.k_out : a.q_out) + (bt * to.b + st * to.t + (lo - begin + sub) * to.h) * kSize + e0;
+      dst_step = to.h * kRows * kSize;
+    }
+    const void *w = kind ? a.wk : a.wq;
+    // element pairs: f[0..1] are the first elements of the lane's four pairs, f[2..3] the second ones
+    auto unpack = [&](piece_t<DT> p0, piece_t<DT> p1, uint64_t (&f)[4]) {
+      float y[8];
+      to_float<DT>(p0, y);
+      to_float<DT>(p1, y + 4);
+      if constexpr (NEIGHBOURS) {
+        f[0] = f2_pack(y[0], y[2]), f[1] = f2_pack(y[4], y[6]), f[2] = f2_pack(y[1], y[3]), f[3] = f2_pack(y[5], y[7]);
+      } else {
+        f[0] = f2_pack(y[0], y[1]), f[1] = f2_pack(y[2], y[3]), f[2] = f2_pack(y[4], y[5]), f[3] = f2_pack(y[6], y[7]);
+      }
+    };
+    uint64_t g[4] = {};
+    if (w && in_row)
+      unpack(load_piece<DT>(static_cast<const char *>(w) + e0, 0), load_piece<DT>(static_cast<const char *>(w) + e1, 0), g);
+#pragma unroll 1
+    for (int row0 = lo; row0 < hi; row0 += kUnroll * kRows) {
+      piece_t<DT> x0[kUnroll], x1[kUnroll];
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int row = row0 + i * kRows;
-      x0[i] = x1[i] = piece_t<DT>{};
-      if (in_row && row < last_row) {
-        const void *src = q;
-        long long at = row * a.sq.h;
-        if (row >= a.Hq) src = k, at = (row - a.Hq) * a.sk.h;
-        if (APPEND && row >= a.Hq + a.Hkv) src = v, at = (row - a.Hq - a.Hkv) * a.sv.h;
-        x0[i] = load_piece<DT>(src, at + e0);
-        x1[i] = load_piece<DT>(src, at + e1);
+      for (int i = 0; i < kUnroll; ++i) {
+        x0[i] = x1[i] = piece_t<DT>{};
+        if (in_row && row0 + i * kRows + sub < hi) {
+          x0[i] = load_piece<DT>(src, 0);
+          x1[i] = load_piece<DT>(src + (e1 - e0), 0);
+        }
+        src += src_step;
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        if (row0 + i * kRows >= hi) break;                // the same for the whole warp
+        uint64_t f[4];
+        unpack(x0[i], x1[i], f);
+        if (w) {
+          uint64_t sq = f2_mul(f[0], f[0]);
+#pragma unroll
+          for (int e = 1; e < 4; ++e) sq = f2_fma(f[e], f[e], sq);
+          const float2 both = f2_unpack(sq);
+          float ss = both.x + both.y;
+#pragma unroll
+          for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
+          const uint64_t r2 = f2_pack(r, r);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[e] = f2_mul(f2_mul(f[e], r2), g[e]);
+        }
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint64_t y1 = f[e], y2 = f[e + 2];
+            f[e] = f2_fma(y2, n2[e], f2_mul(y1, c2[e]));
+            f[e + 2] = f2_fma(y1, s2[e], f2_mul(y2, c2[e]));
+          }
+        }
+        float y[8];
+        {
+          const float2 p = f2_unpack(f[0]), q = f2_unpack(f[1]), v = f2_unpack(f[2]), z = f2_unpack(f[3]);
+          if constexpr (NEIGHBOURS) {
+            y[0] = p.x, y[2] = p.y, y[4] = q.x, y[6] = q.y, y[1] = v.x, y[3] = v.y, y[5] = z.x, y[7] = z.y;
+          } else {
+            y[0] = p.x, y[1] = p.y, y[2] = q.x, y[3] = q.y, y[4] = v.x, y[5] = v.y, y[6] = z.x, y[7] = z.y;
+          }
+        }
+        if (in_row && row0 + i * kRows + sub < hi) {
+          store_piece<DT>(dst, 0, from_float<DT>(y));
+          store_piece<DT>(dst + (e1 - e0), 0, from_float<DT>(y + 4));
+        }
+        dst += dst_step;
       }
     }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int row = row0 + i * kRows;
-      if (row - sub >= last_row) break;                   // the same for the whole warp
-      const bool is_q = row < a.Hq, is_v = APPEND && row >= a.Hq + a.Hkv;
-      float y[8];
-      to_float<DT>(x0[i], y);
-      to_float<DT>(x1[i], y + 4);
-      if (a.wq || a.wk) {                                 // every lane takes part in the sum
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-#pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (is_q ? a.wq != nullptr : a.wk != nullptr) {
-          const float r = rsqrtf(fmaf(ss, a.inv_d, a.eps));
-          float g[8];
-          to_float<DT>(is_q ? wq0 : wk0, g);
-          to_float<DT>(is_q ? wq1 : wk1, g + 4);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = y[e] * r * g[e];
-        }
-      }
-      if (turned) {
-        const float c[4] = {cs[0].x, cs[0].z, cs[1].x, cs[1].z}, s[4] = {cs[0].y, cs[0].w, cs[1].y, cs[1].w};
-        if (a.interleaved) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y1 = y[2 * e], y2 = y[2 * e + 1];
-            y[2 * e] = y1 * c[e] - y2 * s[e];
-            y[2 * e + 1] = y2 * c[e] + y1 * s[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float y1 = y[e], y2 = y[e + 4];
-            y[e] = y1 * c[e] - y2 * s[e];
-            y[e + 4] = y2 * c[e] + y1 * s[e];
-          }
-        }
-      }
-      if (in_row && row < last_row) {
-        void *dst = a.q_out;
-        long long at = bt * a.sqo.b + st * a.sqo.t + row * a.sqo.h;
-        if constexpr (APPEND) {
-          if (!is_q) dst = a.k_pages, at = slot_base + static_cast<long long>(row - a.Hq) * (kPageRows * kCacheD);
-          if (is_v) dst = a.v_pages, at = slot_base + static_cast<long long>(row - a.Hq - a.Hkv) * (kPageRows * kCacheD);
-        } else {
-          if (!is_q) dst = a.k_out, at = bt * a.sko.b + st * a.sko.t + (row - a.Hq) * a.sko.h;
-        }
-        store_piece<DT>(dst, at + e0, is_v ? x0[i] : from_float<DT>(y));
-        store_piece<DT>(dst, at + e1, is_v ? x1[i] : from_float<DT>(y + 4));
-      }
+  }
+  if constexpr (APPEND) {                                 // values: copied as they are
+    const int begin = a.Hq + a.Hkv, lo = max(row_lo, begin), hi = min(row_hi, begin + a.Hkv);
+    const char *src = static_cast<const char *>(a.v) + (st * a.sv.t + (lo - begin + sub) * a.sv.h) * 2 + u * 16;
+    char *dst = static_cast<char *>(a.v_pages) + (slot_base + static_cast<long long>(lo - begin + sub) * (kPageRows * kCacheD)) * 2 + u * 16;
+#pragma unroll 4
+    for (int row = lo + sub; row < hi; row += kRows) {
+      *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+      src += a.sv.h * kRows * 2;
+      dst += static_cast<long long>(kPageRows) * kCacheD * kRows * 2;
     }
   }
 }
@@ -234,15 +268,18 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const Args a, const
 // A warp does all the rows of a token where the tokens alone fill the SMs' warps; with fewer tokens their rows are dealt
 // out, down to one pass per warp, which then computes the token's angles again.
 template <int DT, int G, bool APPEND> int launch_g(const Args &a, long long tokens, int rows, cudaStream_t st) {
-  constexpr int kResident = 148 * 32;
-  const int passes = (rows + 32 / G - 1) / (32 / G);
+  constexpr int kResident = 148 * 32, kRows = 32 / G;
+  const int passes = (rows + kRows - 1) / kRows;
   long long per = tokens * passes / kResident;
   per = per < 1 ? 1 : (per >= passes ? passes : per);
   if (per > kUnroll) per = (per + kUnroll - 1) / kUnroll * kUnroll;
-  const int chunks = static_cast<int>((passes + per - 1) / per);
-  const long long units = tokens * chunks, blocks = (units + kWarps - 1) / kWarps;
-  NB200_REQUIRE(blocks < (1ll << 31), NB200_ERR_UNSUPPORTED, "norm and rotation: too many rows");
-  norm_rope_kernel<DT, G, APPEND><<<dim3(static_cast<unsigned>(blocks)), kThreads, 0, st>>>(a, units, chunks, static_cast<int>(per));
+  const long long chunks = (passes + per - 1) / per, units = tokens * chunks;
+  NB200_REQUIRE(units < (1ll << 31), NB200_ERR_UNSUPPORTED, "norm and rotation: too many rows");
+  const unsigned blocks = static_cast<unsigned>((units + kWarps - 1) / kWarps);
+  if (a.interleaved)
+    norm_rope_kernel<DT, G, APPEND, true><<<blocks, kThreads, 0, st>>>(a, static_cast<unsigned>(units), static_cast<unsigned>(chunks), static_cast<int>(per) * kRows);
+  else
+    norm_rope_kernel<DT, G, APPEND, false><<<blocks, kThreads, 0, st>>>(a, static_cast<unsigned>(units), static_cast<unsigned>(chunks), static_cast<int>(per) * kRows);
   NB200_CHECK_CUDA(cudaGetLastError());
   return NB200_OK;
 }

@@ -9,9 +9,11 @@ from __future__ import annotations
 
 import ctypes
 from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint, c_void_p
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
-from .plugin import find_library_path
+from .plugin import find_binding_path, find_library_path
 
 NB200_OK = 0
 ERROR_NAMES = {-1: "bad argument", -2: "unsupported", -3: "launch failure", -4: "device wait timeout", -5: "NCCL failure"}
@@ -64,11 +66,12 @@ class NativeLibraryError(RuntimeError):
 
 _LIB: ctypes.CDLL | None = None
 _LIB_PATH: Path | None = None
+_BINDING = None
 
 
 def load(path=None) -> ctypes.CDLL:
     """Load (or reload from an explicit path) the kernel library and declare its prototypes."""
-    global _LIB, _LIB_PATH
+    global _BINDING, _LIB, _LIB_PATH
     resolved = find_library_path(path)
     if resolved is None:
         raise NativeLibraryError(
@@ -86,11 +89,40 @@ def load(path=None) -> ctypes.CDLL:
         fn.restype = restype
         fn.argtypes = argtypes
     _LIB, _LIB_PATH = cdll, resolved
+    if _BINDING is not None:
+        _bind(_BINDING)
     return cdll
 
 
 def lib() -> ctypes.CDLL:
     return _LIB if _LIB is not None else load()
+
+
+def _bind(module) -> None:
+    def address(name: str) -> int:
+        return ctypes.cast(getattr(_LIB, name), c_void_p).value
+
+    module.bind(address("nb200_qk_norm_rope"), address("nb200_rope_append"), address("nb200_attn_paged"),
+                _LIB.nb200_attn_paged_workspace_bytes())
+
+
+def binding():
+    """The CPython module ``nb200_torch``, calling the library that ``lib()`` returns."""
+    global _BINDING
+    if _BINDING is None:
+        lib()
+        path = find_binding_path()
+        if path is None:
+            raise NativeLibraryError("the torch binding (nb200_torch.so) was not found; build it with "
+                                     "`python mlir-toy_b200/build_native.py`")
+        import torch  # noqa: F401  (the libraries the module needs)
+
+        loader = importlib.machinery.ExtensionFileLoader("nb200_torch", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nb200_torch", loader))
+        loader.exec_module(module)
+        _bind(module)
+        _BINDING = module
+    return _BINDING
 
 
 def library_path() -> Path | None:

@@ -17,6 +17,7 @@ PLUGIN_PATTERNS = ("libHTileDialectPlugin.*",)
 DEFAULT_LIBRARY_ENV = "NEPTUNE_B200_LIB"
 LIBRARY_PATTERNS = ("libnb200.so", "libnb200.*")
 DEFAULT_FRONT_ENV = "NEPTUNE_HTILE_FRONT_LIB"
+BINDING_PATTERNS = ("nb200_torch.so", "nb200_torch.*")
 FRONT_PATTERNS = ("libhtile_front.so", "libhtile_front.*")
 
 
@@ -64,6 +65,11 @@ def find_library_path(explicit: str | os.PathLike[str] | None = None) -> Path | 
 def find_front_path(explicit: str | os.PathLike[str] | None = None) -> Path | None:
     """Resolve libhtile_front.so (the C++ HTile front end), same search order with $NEPTUNE_HTILE_FRONT_LIB."""
     return _resolve(explicit, DEFAULT_FRONT_ENV, FRONT_PATTERNS)
+
+
+def find_binding_path() -> Path | None:
+    """Resolve nb200_torch.so (the CPython module between torch tensors and the kernel library) in the same directories."""
+    return next((m.resolve() for d in _candidate_dirs() if d.is_dir() and (m := _find_in_dir(d, BINDING_PATTERNS))), None)
 
 
 def find_plugin_path(explicit: str | os.PathLike[str] | None = None) -> Path | None:

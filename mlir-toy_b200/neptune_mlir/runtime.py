@@ -11,8 +11,6 @@ the kernel library every call raises.
 
 from __future__ import annotations
 
-import struct
-
 import torch
 
 from . import native
@@ -61,23 +59,6 @@ def _rows(name: str, t, shape, dtype: str) -> None:
         raise ValueError(f"{name}: rows must be contiguous")
 
 
-def _fits(index: int, dtype, shape, *tensors) -> bool:
-    """Whether all of ``tensors`` are contiguous, on device ``index``, of this dtype and shape.
-
-    The operators of a decode step are called thousands of times a second, so they ask this first (0.3 us a tensor) and
-    go through the checks that name what is wrong (1 us) only if the answer is no.
-    """
-    for t in tensors:
-        if t.dtype is not dtype or t.shape != shape or t.get_device() != index or not t.is_contiguous():
-            return False
-    return True
-
-
-def _fits_rows(index: int, dtype, shape, t) -> bool:
-    """The same for a tensor whose rows alone are contiguous."""
-    return t.dtype is dtype and t.shape == shape and t.get_device() == index and t.stride(-1) == 1
-
-
 def _pools(k_pages, v_pages, Hkv: int, page_size: int, D: int, dtype: str) -> None:
     """Check the two page pools of a paged cache."""
     want = _TORCH_DTYPES[dtype]
@@ -89,18 +70,6 @@ def _pools(k_pages, v_pages, Hkv: int, page_size: int, D: int, dtype: str) -> No
         raise ValueError("k_pages and v_pages must hold the same number of pages")
 
 
-def _launch(fn, what: str, index: int, *args) -> None:
-    """Call a C entry point with device ``index`` current and that device's current stream as the last argument."""
-    stream = torch._C._cuda_getCurrentRawStream(index)   # what torch.cuda.current_stream wraps, without the 2 us
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
-    if rc:
-        native.check(rc, what)
-
-
 def status_buffer(dev: torch.device) -> torch.Tensor:
     """Per-device int32[4] that kernels with bounded device-side waits report into."""
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
@@ -108,12 +77,8 @@ def status_buffer(dev: torch.device) -> torch.Tensor:
     if buf is None:
         buf = torch.zeros(native.STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
         _status_buffers[idx] = buf
+        native.binding().set_status(idx, buf.data_ptr())
     return buf
-
-
-def _status_pointer(index: int) -> int:
-    buf = _status_buffers.get(index)
-    return (status_buffer(torch.device("cuda", index)) if buf is None else buf).data_ptr()
 
 
 def check_status(device=None) -> None:
@@ -236,25 +201,19 @@ def decode_merge_nccl(local_partial, gathered, out, *, rows, D, world, out_dtype
     native.check(rc, "nb200_decode_merge_nccl")
 
 
-def _qk_norm_rope_checks(q, k, positions, inv_freq, q_out, k_out, weights, B, S, Hq, Hkv, D, rot_dim, dtype) -> None:
-    _rows("q", q, (B, S, Hq, D), dtype)
-    _rows("k", k, (B, S, Hkv, D), dtype)
-    _rows("q_out", q_out, (B, Hq, S, D), dtype)
-    _rows("k_out", k_out, (B, Hkv, S, D), dtype)
-    one_row = isinstance(positions, torch.Tensor) and positions.dim() == 1
-    _check("positions", positions, (S,) if one_row else (B, S), torch.int32)
-    _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
-    for name, w in weights.items():
+# The operators of a decode step go through the native binding, which checks the tensors and launches in a few
+# microseconds; it returns None if a tensor is not what the arguments say, and the checks here then say which.
+
+def _refuse(what: str):
+    raise ValueError(f"{what}: the tensors do not fit the arguments")   # the checks before this name the tensor
+
+
+def _weight_checks(weights, D: int, dtype: str) -> list:
+    """Check the norm weights that are there; return them."""
+    there = [(name, w) for name, w in zip(("q_weight", "k_weight"), weights) if w is not None]
+    for name, w in there:
         _check(name, w, (D,), dtype)
-    _same_device(q, k, positions, inv_freq, q_out, k_out, *weights.values())
-
-
-def _weights(q_weight, k_weight) -> dict:
-    """The norm weights that are there."""
-    return {name: w for name, w in (("q_weight", q_weight), ("k_weight", k_weight)) if w is not None}
-
-
-_PACK_8, _PACK_13, _PACK_4 = (struct.Struct(f"={n}q").pack for n in (8, 13, 4))
+    return [w for _, w in there]
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_out, k_out, q_weight=None, k_weight=None, *, B, S, Hq, Hkv, D, rot_dim,
@@ -266,23 +225,21 @@ def qk_norm_rope(q, k, positions, inv_freq, q_out, k_out, q_weight=None, k_weigh
     multiples of 16 bytes (so an output may also be its input's ``transpose(1, 2)``, in place).  positions is int32
     [S] or [B, S], inv_freq fp32 [rot_dim / 2]; the weights are [D].
     """
-    weights = _weights(q_weight, k_weight)
-    try:
-        want, index, one_row = _TORCH_DTYPES[dtype], q.get_device(), positions.dim() == 1
-        fine = (index >= 0 and _fits_rows(index, want, (B, S, Hq, D), q) and _fits_rows(index, want, (B, S, Hkv, D), k)
-                and _fits_rows(index, want, (B, Hq, S, D), q_out) and _fits_rows(index, want, (B, Hkv, S, D), k_out)
-                and _fits(index, torch.int32, (S,) if one_row else (B, S), positions)
-                and _fits(index, torch.float32, (rot_dim // 2,), inv_freq) and _fits(index, want, (D,), *weights.values()))
-    except AttributeError:
-        fine = False
-    if not fine:
-        _qk_norm_rope_checks(q, k, positions, inv_freq, q_out, k_out, weights, B, S, Hq, Hkv, D, rot_dim, dtype)
-    qs, ks, qo, ko = q.stride(), k.stride(), q_out.stride(), k_out.stride()
-    strides = _PACK_13(qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qo[0], qo[2], qo[1], ko[0], ko[2], ko[1], 0 if one_row else S)
-    _launch(native.lib().nb200_qk_norm_rope, "nb200_qk_norm_rope", index, q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
-            k_out.data_ptr(), positions.data_ptr(), inv_freq.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
-            None if k_weight is None else k_weight.data_ptr(), strides, B, S, Hq, Hkv, D, rot_dim, int(interleaved), eps,
-            native.DTYPE_CODES[dtype])
+    rc = native.binding().qk_norm_rope(q, k, positions, inv_freq, q_out, k_out, q_weight, k_weight, B, S, Hq, Hkv, D,
+                                       rot_dim, interleaved, eps, native.DTYPE_CODES[dtype])
+    if rc == 0:
+        return
+    if rc is None:
+        _rows("q", q, (B, S, Hq, D), dtype)
+        _rows("k", k, (B, S, Hkv, D), dtype)
+        _rows("q_out", q_out, (B, Hq, S, D), dtype)
+        _rows("k_out", k_out, (B, Hkv, S, D), dtype)
+        one_row = isinstance(positions, torch.Tensor) and positions.dim() == 1
+        _check("positions", positions, (S,) if one_row else (B, S), torch.int32)
+        _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
+        _same_device(q, k, positions, inv_freq, q_out, k_out, *_weight_checks((q_weight, k_weight), D, dtype))
+        _refuse("qk_norm_rope")
+    native.check(rc, "nb200_qk_norm_rope")
 
 
 def _paged_checks(k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D, dtype) -> None:
@@ -290,12 +247,6 @@ def _paged_checks(k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, m
     _check("block_table", block_table, (B, max_pages), torch.int32)
     _check("cu_seqlens", cu_seqlens, (B + 1,), torch.int32)
     _check("seq_lens", seq_lens, (B,), torch.int32)
-
-
-def _paged_fit(index, want, k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D) -> bool:
-    return (_fits(index, want, (k_pages.shape[0], Hkv, page_size, D), k_pages, v_pages)
-            and _fits(index, torch.int32, (B, max_pages), block_table) and _fits(index, torch.int32, (B + 1,), cu_seqlens)
-            and _fits(index, torch.int32, (B,), seq_lens))
 
 
 def rope_append(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, q_out, q_weight=None,
@@ -307,37 +258,29 @@ def rope_append(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, in
     Rows of D are contiguous, the other strides free multiples of 16 bytes; q_out may be q.  Positions or pages that
     the table or the pool does not have are reported by ``check_status``.
     """
-    weights = _weights(q_weight, k_weight)
-    if Hq == 0 and not (q is None and q_out is None):
-        raise ValueError("rope_append: Hq = 0 goes with q = q_out = None")
-    try:
-        want, index = _TORCH_DTYPES[dtype], k.get_device()
-        fine = (index >= 0 and _fits_rows(index, want, (T, Hkv, D), k) and _fits_rows(index, want, (T, Hkv, D), v)
-                and (Hq == 0 or (_fits_rows(index, want, (T, Hq, D), q) and _fits_rows(index, want, (T, Hq, D), q_out)))
-                and _paged_fit(index, want, k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D)
-                and _fits(index, torch.float32, (rot_dim // 2,), inv_freq) and _fits(index, want, (D,), *weights.values()))
-    except AttributeError:
-        fine = False
-    if not fine:
-        if Hq != 0:
+    args = (q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, q_out, q_weight, k_weight, T, B, Hq,
+            Hkv, max_pages, page_size, D, rot_dim, interleaved, eps, native.DTYPE_CODES[dtype])
+    rc = native.binding().rope_append(*args)
+    if rc == 0:
+        return
+    if rc is None:
+        if Hq == 0:
+            if q is not None or q_out is not None:
+                raise ValueError("rope_append: Hq = 0 goes with q = q_out = None")
+        else:
             _rows("q", q, (T, Hq, D), dtype)
             _rows("q_out", q_out, (T, Hq, D), dtype)
         _rows("k", k, (T, Hkv, D), dtype)
         _rows("v", v, (T, Hkv, D), dtype)
         _paged_checks(k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D, dtype)
         _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
-        for name, w in weights.items():
-            _check(name, w, (D,), dtype)
-        _same_device(k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq, *weights.values(),
-                     *((q, q_out) if Hq else ()))
-    qs, ks, vs, qo = q.stride() if Hq else (0, 0), k.stride(), v.stride(), q_out.stride() if Hq else (0, 0)
-    strides = _PACK_8(qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], qo[0], qo[1])
-    _launch(native.lib().nb200_rope_append, "nb200_rope_append", index, q.data_ptr() if Hq else None, k.data_ptr(),
-            v.data_ptr(), q_out.data_ptr() if Hq else None, k_pages.data_ptr(), v_pages.data_ptr(),
-            block_table.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), inv_freq.data_ptr(),
-            None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), strides, T,
-            B, Hq, Hkv, k_pages.shape[0], max_pages, page_size, D, rot_dim, int(interleaved), eps,
-            native.DTYPE_CODES[dtype], _status_pointer(index))
+        dev = _same_device(k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq,
+                           *_weight_checks((q_weight, k_weight), D, dtype), *((q, q_out) if Hq else ()))
+        status_buffer(dev)                                       # the first call on a device makes its status words
+        rc = native.binding().rope_append(*args)
+        if rc is None:
+            _refuse("rope_append")
+    native.check(rc, "nb200_rope_append")
 
 
 def attn_paged_workspace_bytes() -> int:
@@ -352,16 +295,12 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace
     q, out [T, Hq, D] with contiguous rows and token and head strides that are multiples of 16 bytes; workspace is a
     uint8 tensor of attn_paged_workspace_bytes(), one for each call that can run at the same time.
     """
-    lib = native.lib()
-    try:
-        want, index = _TORCH_DTYPES[dtype], q.get_device()
-        fine = (index >= 0 and _fits_rows(index, want, (T, Hq, D), q) and _fits_rows(index, want, (T, Hq, D), out)
-                and _paged_fit(index, want, k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D)
-                and workspace.get_device() == index and workspace.is_contiguous()
-                and workspace.nbytes >= lib.nb200_attn_paged_workspace_bytes())
-    except AttributeError:
-        fine = False
-    if not fine:
+    args = (q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out, T, B, Hq, Hkv, max_pages, page_size, D,
+            native.DTYPE_CODES[dtype], scale_log2)
+    rc = native.binding().attn_paged(*args)
+    if rc == 0:
+        return
+    if rc is None:
         _rows("q", q, (T, Hq, D), dtype)
         _rows("out", out, (T, Hq, D), dtype)
         _paged_checks(k_pages, v_pages, block_table, cu_seqlens, seq_lens, B, Hkv, max_pages, page_size, D, dtype)
@@ -369,12 +308,11 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace
         if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
                 and workspace.numel() * workspace.element_size() >= need):
             raise ValueError(f"workspace: need a contiguous CUDA tensor of at least {need} bytes")
-        _same_device(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out)
-    qs, outs = q.stride(), out.stride()
-    _launch(lib.nb200_attn_paged, "nb200_attn_paged", index, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-            block_table.data_ptr(), cu_seqlens.data_ptr(), seq_lens.data_ptr(), workspace.data_ptr(), out.data_ptr(),
-            _PACK_4(qs[0], qs[1], outs[0], outs[1]), T, B, Hq, Hkv, k_pages.shape[0], max_pages, page_size, D,
-            native.DTYPE_CODES[dtype], scale_log2, _status_pointer(index))
+        status_buffer(_same_device(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out))
+        rc = native.binding().attn_paged(*args)
+        if rc is None:
+            _refuse("attn_paged")
+    native.check(rc, "nb200_attn_paged")
 
 
 def selective_scan(u, delta, A, Bm, Cm, Dskip, z, out, *, B, Dm, L, N, dtype) -> None:
