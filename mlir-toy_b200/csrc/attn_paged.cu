@@ -17,11 +17,18 @@
 //   S(g) = Q K(g)^T      8 x tcgen05.mma 128x128x16, both operands in shared memory, into TMEM buffer g % 3
 //   softmax(g)           warpgroup g & 1 (thread = row = TMEM lane): scores to registers, row maximum, p = 2^(s - m),
 //                        P(g) as packed 16-bit over the first 64 columns of the same TMEM buffer
-//   O += P(g) V(g)       8 x tcgen05.mma 128x128x16 with P read from TMEM, O in TMEM columns 384..511
+//   O += P(g) V(g)       8 x tcgen05.mma 128x128x16 with P read from TMEM
 //
 //   warps 0-3 / 4-7  softmax of even / odd blocks      warps 8-11   epilogue
 //   warp 12, 15      TMA producers: Q and K (and the list of tiles); V (warp 15 also allocates the 512 TMEM columns)
 //   warp 13, 14      issuers of the score products and of the PV products (one lane each)
+//
+// The 512 TMEM columns are four regions of 128: three score buffers and O.  Reading a finished O takes the epilogue 2 to 3
+// us, and a tile of a chunk may be over in two blocks, so the next tile does not wait for it: its O takes over the region
+// of the score buffer whose turn comes last, and that buffer moves to the old O's region once it has been read, two blocks
+// later.  (Waiting cost 4.5 us a tile: 223 us for a 4096-token first chunk.)  What bounds a block then is the chain from
+// PV(g-3) over S(g) and its softmax to PV(g), 2.6 us for three blocks in flight; a third stage for K and V in place of
+// Q's second buffer changed nothing.
 //
 // P is rounded to the storage type because the second product takes both operands in one 16-bit type; the row sum adds
 // the unrounded values.  The running maximum passes between the warpgroups through shared memory, O is rescaled only when
@@ -30,14 +37,16 @@
 // What is masked.  A table entry that is not needed or not in the pool becomes a coordinate outside the tensor map, which
 // TMA fills with zeros; nothing outside the pool is addressed.  Scores of hidden columns are replaced, not added to, so K
 // may hold anything there.  V may not, since 0 * NaN is NaN: in the blocks that some row of the tile does not see
-// whole, the softmax warps clear V rows behind the sequence's end in shared memory, and look for infinities and NaN in the
-// rows that only some of the tile's rows see.  Such a value is replaced by 0 and noted; the epilogue makes it a NaN in
-// exactly those rows that see it.
+// whole, the epilogue warps (idle then) clear V rows behind the sequence's end in shared memory, and look for infinities
+// and NaN in the rows that only some of the tile's rows see, before the PV product of that block.  Such a value is
+// replaced by 0 and noted; the epilogue makes it a NaN in exactly those rows that see it.  Done by the softmax warps, the
+// same look cost 44 of 211 us at a 4096-token first chunk.
 //
 // Every wait is bounded; on expiry the CTA records a code in the status words and unwinds.
 #include <cuda.h>
 
 #include <atomic>
+#include <cstddef>
 
 #include "nb200_common.cuh"
 #include "sm100_primitives.cuh"
@@ -57,11 +66,11 @@ constexpr int kTileBytes = 128 * kD * 2;        // 32 KB: two halves of 64 colum
 constexpr int kBox = kTileBytes / 2;
 constexpr int kPageBox = kPageRows * 128;       // one page's half: 8 KB
 constexpr int kSBufs = 3;
-constexpr int kTmemCols = 512;                  // S/P 0 | S/P 1 | S/P 2 | O, 128 columns each
-constexpr int kTmemO = 384;
+constexpr int kTmemCols = 512;                  // four regions of 128 columns
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kSched = 16;                      // ring of tile descriptors handed from the K producer to the other roles
 constexpr int kMaxCtas = 160;                   // CTAs that the workspace has room for
+constexpr int kTileUnits = 1;                   // what changing tiles costs, in blocks, on the line that is cut
 
 enum : int { kErrProducer = 41, kErrMma = 42, kErrSoftmax = 43, kErrEpilogue = 44, kErrTable = 22, kErrSlot = 23 };
 
@@ -73,6 +82,7 @@ struct Segment {
   int pos0;                  // position of the first token
   int len;                   // rows of the sequence's cache
   int blk0, nblk;            // KV blocks
+  int check;                 // blocks from this one on (of nblk) have V rows that not every row of the tile sees
   int slot;                  // -1: the whole tile; 0 / 1: partial that ends / begins a tile
 };
 // Tile that begins in a CTA and goes on in the next ones.
@@ -97,21 +107,25 @@ constexpr size_t kPartMl = static_cast<size_t>(kMaxCtas) * 2 * kBM * sizeof(floa
 struct Shared {
   uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[kSBufs], p_full[kSBufs], pv_done[kSBufs];
-  uint64_t o_full, o_free, m_ready[2], lm_ready, lm_free;
+  uint64_t o_full[4], o_free[4], m_ready[2], lm_ready[2], lm_free[2], notes_read;
+  uint64_t look[2], looked[2];       // V of a block to be looked through is on its way / has been looked through, per stage
   uint64_t sched_full[kSched];
   unsigned long long taint[2][kD];   // per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is not finite)
-  long long scan[kThreads / 32];
-  long long first_block, last_block, total;
+  unsigned scan[kThreads / 32];
+  unsigned before;                  // units in front of the sequence that the CTA's range begins in
   Segment seg[kSched];
-  int start_b, start_h, start_j, start_blk;
+  int start_b;
   int taint_any[2];                  // tile number + 1
   uint32_t tmem_base;
   int abort_flag;
   int skip;
   float mslot[2][kBM];               // running maximum decided by block g, slot g & 1
-  float lm[2][kBM][2];               // per warpgroup: (maximum last used, partial row sum) of the finished tile
+  float2 lm[2][2][kBM];              // of tile n in [n & 1], per warpgroup: (maximum last used, partial row sum)
 };
-constexpr int kSmemBytes = 6 * kTileBytes + 1024 + static_cast<int>(sizeof(Shared));
+constexpr int kStage = 32 * 64;      // a warp's 32 rows of 64 bytes on their way out
+constexpr int kOffStage = 6 * kTileBytes, kOffShared = kOffStage + 4 * kStage;
+constexpr int kSmemBytes = kOffShared + 1024 + static_cast<int>(sizeof(Shared));
+static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
 
 __device__ __forceinline__ void report(int *status, int code, int detail) {
   if (status && atomicCAS(status, 0, code) == 0) {
@@ -139,13 +153,33 @@ __device__ __forceinline__ Seq seq_of(const Args &a, int b) {
 // KV blocks of the tile that starts at token j0 of the sequence: what its last token sees, at least one.
 __device__ __forceinline__ int tile_blocks(const Seq &s, int j0, int tok_tile) {
   const int sees = min(s.pos + min(s.n, j0 + tok_tile), s.len);
-  return sees <= 0 ? 1 : (sees + kBN - 1) / kBN;
+  return max((sees + kBN - 1) >> 7, 1);
 }
-__device__ __forceinline__ long long seq_blocks(const Seq &s, int tok_tile) {
-  long long sum = 0;
-  for (int j0 = 0; j0 < s.n; j0 += tok_tile) sum += tile_blocks(s, j0, tok_tile);
+// Units of a sequence's tiles for one kv head, those of tiles first, first + step, ...
+__device__ __forceinline__ unsigned seq_units(const Seq &s, int tok_tile, int first, int step) {
+  unsigned sum = 0;
+#pragma unroll 1
+  for (int j0 = first * tok_tile; j0 < s.n; j0 += step * tok_tile) sum += tile_blocks(s, j0, tok_tile) + kTileUnits;
   return sum;
 }
+__device__ __forceinline__ unsigned warp_scan(unsigned x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned up = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += up;
+  }
+  return x;
+}
+
+// Which TMEM region the three score buffers (bytes 0 to 2) and O (byte 3) are in.  Tile n > 0, whose first block is g,
+// takes the region of buffer (g + 2) % 3 for its O and leaves its predecessor's to that buffer.
+constexpr uint32_t kRegions = 0x03020100u;
+__device__ __forceinline__ uint32_t next_regions(uint32_t map, int g) {
+  const int sh = 8 * ((g + 2) % kSBufs);
+  const uint32_t o = map >> 24, s = (map >> sh) & 0xffu;
+  return (map & ~(0xff000000u | (0xffu << sh))) | (s << 24) | (o << sh);
+}
+__device__ __forceinline__ uint32_t region(uint32_t map, int i) { return ((map >> (8 * i)) & 0xffu) * 128u; }   // its first column
 
 // fma(x, 0, acc) on packed 16-bit pairs: stays 0 while every x is finite, becomes NaN for good otherwise.
 template <int DT> __device__ __forceinline__ uint32_t finite_probe(uint32_t x, uint32_t acc) {
@@ -171,51 +205,53 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t sQ = base;                                   // buffer n & 1 of tile n
   const uint32_t sK = base + 2 * kTileBytes;                  // stage g & 1
   const uint32_t sV = base + 4 * kTileBytes;
-  Shared *sh = reinterpret_cast<Shared *>(smem + 6 * kTileBytes);
+  Shared *sh = reinterpret_cast<Shared *>(smem + kOffShared);
   volatile int *abort_flag = &sh->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 2 * kD) sh->taint[threadIdx.x / kD][threadIdx.x % kD] = 0;
+  if (warp == 15) {
+    tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 14 && lane == 0) {
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
     sh->abort_flag = 0;
+    sh->start_b = 0;
+    sh->before = 0;
+    sh->taint_any[0] = sh->taint_any[1] = 0;
     const int code = a.status ? *reinterpret_cast<volatile int *>(a.status) : 0;
     sh->skip = (code != 0 && code != kErrTable && code != kErrSlot) ? 1 : 0;   // an expired wait, not refused data
     a.owners[blockIdx.x].parts = 0;
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(smem_u32(&sh->q_full[b]), 1);
-      mbar_init(smem_u32(&sh->q_empty[b]), 1);
-      mbar_init(smem_u32(&sh->k_full[b]), 1);
-      mbar_init(smem_u32(&sh->k_empty[b]), 1);
-      mbar_init(smem_u32(&sh->v_full[b]), 1);
-      mbar_init(smem_u32(&sh->v_empty[b]), 1);
-      mbar_init(smem_u32(&sh->m_ready[b]), 128);
-      sh->taint_any[b] = 0;
+  }
+  if (warp == 13) {
+    // one barrier per lane and turn
+    uint64_t *const bars = sh->q_full;
+    constexpr int kBars = (offsetof(Shared, taint) - offsetof(Shared, q_full)) / sizeof(uint64_t);
+    for (int i = lane; i < kBars; i += 32) {
+      uint64_t *const bar = bars + i;
+      uint32_t count = 1;
+      if ((bar >= sh->p_full && bar < sh->p_full + kSBufs) || (bar >= sh->o_free && bar < sh->o_free + 4) || bar == &sh->notes_read || (bar >= sh->m_ready && bar < sh->m_ready + 2) ||
+          (bar >= sh->lm_free && bar < sh->lm_free + 2) || (bar >= sh->looked && bar < sh->looked + 2))
+        count = 128;
+      if (bar >= sh->lm_ready && bar < sh->lm_ready + 2) count = 256;
+      mbar_init(smem_u32(bar), count);
     }
-    for (int b = 0; b < kSBufs; ++b) {
-      mbar_init(smem_u32(&sh->s_full[b]), 1);
-      mbar_init(smem_u32(&sh->p_full[b]), 128);
-      mbar_init(smem_u32(&sh->pv_done[b]), 1);
-    }
-    mbar_init(smem_u32(&sh->o_full), 1);
-    mbar_init(smem_u32(&sh->o_free), 128);
-    mbar_init(smem_u32(&sh->lm_ready), 256);
-    mbar_init(smem_u32(&sh->lm_free), 128);
-    for (int b = 0; b < kSched; ++b) mbar_init(smem_u32(&sh->sched_full[b]), 1);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  if (threadIdx.x < 2 * kD) sh->taint[threadIdx.x / kD][threadIdx.x % kD] = 0;
 
-  // ---- the CTA's range of the line of blocks: a scan over the sequences' block counts, a thread per sequence ----
-  auto scan = [&](int b0, long long &running, long long &before) -> long long {
+  // ---- the CTA's range of the line: the units in front of each sequence ----
+  // Up to 16 sequences: a warp each, its lanes over the tiles.  More: a thread per sequence and a scan, chunk by chunk.
+  const bool few = a.B <= kThreads / 32;
+  unsigned total = 0, before = 0, mine = 0;
+  auto scan = [&](int b0, unsigned &running) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    const long long mine = b < a.B ? seq_blocks(seq_of(a, b), a.tok_tile) * a.Hkv : 0;
-    long long incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
+    mine = b < a.B ? seq_units(seq_of(a, b), a.tok_tile, 0, 1) * a.Hkv : 0;
+    const unsigned incl = warp_scan(mine, lane);
     __syncthreads();
     if (lane == 31) sh->scan[warp] = incl;
     __syncthreads();
@@ -224,68 +260,67 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (w < warp) before += sh->scan[w];
       running += sh->scan[w];
     }
-    return mine;
   };
-  long long total = 0, before = 0, mine = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) mine = scan(b0, total, before);
-  const int ctas = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-  if (sh->skip || static_cast<int>(blockIdx.x) >= ctas) return;   // the same for every thread of the CTA
-  const long long r0 = total * blockIdx.x / ctas, r1 = total * (blockIdx.x + 1) / ctas;
-  auto locate = [&](int b) {   // the thread whose sequence holds block r0 finds kv head, tile and block in it
-    if (before > r0 || r0 >= before + mine) return;
-    const Seq s = seq_of(a, b);
-    const long long per_head = mine / a.Hkv;
-    long long rem = r0 - before;
-    sh->start_b = b;
-    sh->start_h = static_cast<int>(rem / per_head);
-    rem %= per_head;
-    int j0 = 0;
-    for (int n; rem >= (n = tile_blocks(s, j0, a.tok_tile)); j0 += a.tok_tile) rem -= n;
-    sh->start_j = j0;
-    sh->start_blk = static_cast<int>(rem);
-  };
-  if (a.B <= kThreads) {
-    locate(threadIdx.x);
-  } else {
-    long long running = 0;
-    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-      mine = scan(b0, running, before);
-      locate(b0 + static_cast<int>(threadIdx.x));
+  if (few) {
+    const unsigned sum = warp_scan(warp < a.B ? seq_units(seq_of(a, warp), a.tok_tile, lane, 32) : 0, lane);
+    if (lane == 31) sh->scan[warp] = mine = sum * a.Hkv;
+    __syncthreads();
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w == warp) before = total;
+      total += sh->scan[w];
     }
+  } else {
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) scan(b0, total);
   }
-
-  if (warp == 15) {
-    tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
-    tmem_relinquish();
-  }
-  if (warp == 12 && lane == 0) {
-    tma_prefetch_desc(&tm_q);
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
+  // CTA c takes `share` units, and one more if c < more_until
+  const unsigned ctas = min(gridDim.x, total), share = total / max(ctas, 1u), more_until = total - share * ctas;
+  const bool idle = sh->skip || blockIdx.x >= ctas;            // the same for every thread of the CTA
+  const unsigned r0 = share * blockIdx.x + min(blockIdx.x, more_until), r1 = r0 + share + (blockIdx.x < more_until ? 1 : 0);
+  auto claim = [&](int b) {                                    // the thread whose sequence holds unit r0
+    if (idle || before > r0 || r0 >= before + mine) return;
+    sh->start_b = b;
+    sh->before = before;
+  };
+  if (few) {
+    if (lane == 31) claim(warp);
+  } else if (a.B <= kThreads) {
+    claim(threadIdx.x);
+  } else {
+    unsigned running = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+      scan(b0, running);
+      claim(b0 + static_cast<int>(threadIdx.x));
+    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh->tmem_base;
+  if (idle) {
+    if (warp == 15) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
 
   const uint32_t b_q_full = smem_u32(&sh->q_full[0]), b_q_empty = smem_u32(&sh->q_empty[0]),
                  b_k_full = smem_u32(&sh->k_full[0]), b_k_empty = smem_u32(&sh->k_empty[0]),
                  b_v_full = smem_u32(&sh->v_full[0]), b_v_empty = smem_u32(&sh->v_empty[0]),
                  b_s_full = smem_u32(&sh->s_full[0]), b_p_full = smem_u32(&sh->p_full[0]),
-                 b_pv_done = smem_u32(&sh->pv_done[0]), b_o_full = smem_u32(&sh->o_full),
-                 b_o_free = smem_u32(&sh->o_free), b_m_ready = smem_u32(&sh->m_ready[0]),
-                 b_lm_ready = smem_u32(&sh->lm_ready), b_lm_free = smem_u32(&sh->lm_free),
+                 b_pv_done = smem_u32(&sh->pv_done[0]), b_o_full = smem_u32(&sh->o_full[0]),
+                 b_o_free = smem_u32(&sh->o_free[0]), b_notes_read = smem_u32(&sh->notes_read), b_m_ready = smem_u32(&sh->m_ready[0]),
+                 b_lm_ready = smem_u32(&sh->lm_ready[0]), b_lm_free = smem_u32(&sh->lm_free[0]),
+                 b_look = smem_u32(&sh->look[0]), b_looked = smem_u32(&sh->looked[0]),
                  b_sched = smem_u32(&sh->sched_full[0]);  // element i at + 8 * i
 
-  // The K producer lists the CTA's tiles in a ring that every other role reads.  The roles are never more than 7 tiles
-  // apart (2 Q buffers, 3 score buffers, one O), so 16 slots need no "empty" barrier.  Null: an expired wait.
+  // The K producer lists the CTA's tiles in a ring that every other role reads.  The roles are never more than 10 tiles
+  // apart (two Q buffers, two stages, three score buffers, O's of three tiles), so 16 slots need no "empty" barrier.
+  // Null: an expired wait.
   auto segment_at = [&](int n) -> const volatile Segment * {
     if (!mbar_wait(b_sched + 8 * (n % kSched), (n / kSched) & 1, abort_flag)) return nullptr;
     return &sh->seg[n % kSched];
   };
 
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp == 12 || warp == 15) {
       // ================================ TMA producers ================================
       // warp 12: the list of tiles, Q of every tile and the K blocks; warp 15: the V blocks.  Lane i reads the table
@@ -293,92 +328,124 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const bool is_k = warp == 12;
       const CUtensorMap *tm = is_k ? &tm_k : &tm_v;
       const uint32_t s_dst = is_k ? sK : sV, b_full = is_k ? b_k_full : b_v_full, b_empty = is_k ? b_k_empty : b_v_empty;
+      const uint32_t q_bytes = a.group * a.tok_tile * 256;
       const int outside = a.num_pages * a.Hkv;             // a slice that the tensor map does not have: zeros
-      const int q_bytes = a.group * a.tok_tile * 256;
-      int sb = sh->start_b, shd = sh->start_h, sj = sh->start_j, sblk = sh->start_blk;   // the scheduler's place
-      long long at = r0;
-      bool ok = true;
-      int g = 0, issued = 0, q_issued = 0;
-      for (int n = 0; ok; ++n) {
-        if (is_k) {
-          if (lane == 0) {
-            Segment w{};
-            if (at < r1) {
-              Seq s = seq_of(a, sb);
-              if (sj >= s.n) {                             // on to the next kv head, or sequence with new tokens
-                sj = 0;
-                if (++shd == a.Hkv) {
-                  shd = 0;
-                  do s = seq_of(a, ++sb); while (s.n == 0 && sb < a.B - 1);   // at < r1: there is one
-                }
-              }
-              const int blocks = tile_blocks(s, sj, a.tok_tile);
-              const int take = static_cast<int>(min(static_cast<long long>(blocks - sblk), r1 - at));
-              w.more = 1;
-              w.b = sb, w.kvh = shd;
-              w.tok0 = s.first + sj, w.ntok = min(a.tok_tile, s.n - sj);
-              w.pos0 = s.pos + sj, w.len = s.len;
-              w.blk0 = sblk, w.nblk = take;
-              w.slot = take == blocks ? -1 : (sblk > 0 ? 0 : 1);
-              if (w.slot == 1) {                           // goes on in the CTAs up to the one that has its last block
-                const long long end = at + blocks;
-                const int last = static_cast<int>((end * ctas + total - 1) / total) - 1;
-                a.owners[blockIdx.x] = Owner{last - static_cast<int>(blockIdx.x) + 1, w.kvh, w.tok0, w.ntok};
-              }
-              at += take;
-              sblk += take;
-              if (sblk == blocks) {
-                sblk = 0;
-                sj += a.tok_tile;
+      // the scheduler's place: sequence, kv head, first token of the tile, block in it
+      int sb = 0, shd = 0, sj = 0, sblk = 0;
+      unsigned at = r0;
+      Seq seq{};
+      if (is_k) {
+        sb = sh->start_b;
+        seq = seq_of(a, sb);
+        unsigned rem = r0 - sh->before;
+        const unsigned sum = __shfl_sync(0xffffffffu, warp_scan(seq_units(seq, a.tok_tile, lane, 32), lane), 31);
+        shd = static_cast<int>(rem / max(sum, 1u));
+        rem -= shd * sum;
+        if (static_cast<unsigned>(shd) >= static_cast<unsigned>(a.Hkv)) at = r1;   // cu_seqlens is not a running sum: nothing to do
+        for (;; sj += 32 * a.tok_tile) {                   // 32 tiles at a time
+          const int j0 = sj + lane * a.tok_tile;
+          const unsigned units = j0 < seq.n ? tile_blocks(seq, j0, a.tok_tile) + kTileUnits : 0;
+          const unsigned incl = warp_scan(units, lane);
+          const unsigned past = __ballot_sync(0xffffffffu, incl > rem);
+          if (past) {
+            const int hit = __ffs(past) - 1;
+            sj += hit * a.tok_tile;
+            sblk = static_cast<int>(rem - __shfl_sync(0xffffffffu, incl - units, hit));
+            break;
+          }
+          rem -= __shfl_sync(0xffffffffu, incl, 31);
+          if (sj >= seq.n) break;                          // cannot be: rem is below the head's units
+        }
+      }
+      auto list_next = [&](int n) {                        // lane 0 of the K producer: tile n goes into the ring
+        Segment w{};
+        while (at < r1) {
+          if (sj >= seq.n) {                               // on to the next kv head, or sequence with new tokens
+            sj = 0;
+            if (++shd == a.Hkv) {
+              shd = 0;
+              do {
+                if (++sb < a.B) seq = seq_of(a, sb);
+              } while (seq.n == 0 && sb < a.B);
+              if (sb >= a.B) {                             // not with a running sum in cu_seqlens
+                at = r1;
+                break;
               }
             }
-            sh->seg[n % kSched] = w;
-            mbar_arrive(b_sched + 8 * (n % kSched));
           }
-          __syncwarp();
+          const int blocks = tile_blocks(seq, sj, a.tok_tile);
+          if (sblk < blocks) {
+            const int take = static_cast<int>(min(static_cast<unsigned>(blocks - sblk), r1 - at));
+            w.more = 1;
+            w.b = sb, w.kvh = shd;
+            w.tok0 = seq.first + sj, w.ntok = min(a.tok_tile, seq.n - sj);
+            w.pos0 = seq.pos + sj, w.len = seq.len;
+            w.blk0 = sblk, w.nblk = take;
+            w.check = max(max(min(w.pos0 + 1, w.len), 0) / kBN - sblk, 0);
+            w.slot = take == blocks ? -1 : (sblk > 0 ? 0 : 1);
+            if (w.slot == 1) {                             // goes on in the CTAs up to the one that has its last block
+              const unsigned x = at + blocks - 1, longer = more_until * (share + 1);
+              const unsigned last = x < longer ? x / (share + 1) : more_until + (x - longer) / share;
+              a.owners[blockIdx.x] = Owner{static_cast<int>(last - blockIdx.x) + 1, w.kvh, w.tok0, w.ntok};
+            }
+            at += take;
+            sblk += take;
+          }
+          if (sblk >= blocks) {                            // the tile's blocks are dealt out: the rest of its units is nobody's
+            at += blocks + kTileUnits - sblk;
+            sblk = 0;
+            sj += a.tok_tile;
+          }
+          if (w.more) break;
         }
+        sh->seg[n % kSched] = w;
+        mbar_arrive(b_sched + 8 * (n % kSched));
+      };
+      int kvh = 0, blk0 = 0, pages = 0;
+      const int *table = nullptr;
+      auto slice_of = [&](int j) -> int {                  // of page (2 * (blk0 + j) + lane): its slice of the pool's map
+        const int page = 2 * (blk0 + j) + lane;
+        if (page >= pages) return outside;
+        const int e = table[page];
+        if (e >= 0 && e < a.num_pages) return e * a.Hkv + kvh;
+        if (is_k) report(a.status, kErrTable, e);
+        return outside;
+      };
+      bool ok = true;
+      int g = 0, issued = 0, q_issued = 0;
+      for (int n = 0;; ++n) {
+        // the next tile's lengths and table entries are fetched while the ring of blocks is full
+        if (is_k && lane == 0) list_next(n);
+        __syncwarp();
         const volatile Segment *seg = segment_at(n);
-        if (!__all_sync(0xffffffffu, seg != nullptr)) {
-          if (lane == 0) report(a.status, kErrProducer, -1000 - n);
-          ok = false;
-          break;
-        }
-        if (!seg->more) break;
-        const int kvh = seg->kvh, blk0 = seg->blk0, nblk = seg->nblk;
-        const int pages = min((seg->len + kPageRows - 1) / kPageRows, 2 * (blk0 + nblk));   // needed here
-        const int *table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
+        ok = __all_sync(0xffffffffu, seg != nullptr);
+        if (!ok || !seg->more) break;
+        kvh = seg->kvh, blk0 = seg->blk0;
+        const int nblk = seg->nblk, check = seg->check;
+        pages = min((seg->len + kPageRows - 1) / kPageRows, 2 * (blk0 + nblk));   // needed here
+        table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
+        int next = slice_of(0);
         if (is_k && lane == 0) {
           ok = mbar_wait(b_q_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag);
-          if (!ok) {
-            report(a.status, kErrProducer, -1 - n);
-          } else {
+          if (ok) {
+            const int tok0 = seg->tok0;
             mbar_arrive_expect_tx(b_q_full + 8 * (n & 1), q_bytes);
-            tma_load_3d(sQ + (n & 1) * kTileBytes, &tm_q, 0, kvh * a.group, seg->tok0, b_q_full + 8 * (n & 1));
-            tma_load_3d(sQ + (n & 1) * kTileBytes + kBox, &tm_q, 64, kvh * a.group, seg->tok0, b_q_full + 8 * (n & 1));
+            tma_load_3d(sQ + (n & 1) * kTileBytes, &tm_q, 0, kvh * a.group, tok0, b_q_full + 8 * (n & 1));
+            tma_load_3d(sQ + (n & 1) * kTileBytes + kBox, &tm_q, 64, kvh * a.group, tok0, b_q_full + 8 * (n & 1));
             ++q_issued;
           }
         }
         ok = __all_sync(0xffffffffu, ok);
-        auto slice_of = [&](int j) -> int {                // of page (2 * (blk0 + j) + lane): its slice of the pool's map
-          const int page = 2 * (blk0 + j) + lane;
-          if (page >= pages) return outside;
-          const int e = table[page];
-          if (e >= 0 && e < a.num_pages) return e * a.Hkv + kvh;
-          if (is_k) report(a.status, kErrTable, e);
-          return outside;
-        };
-        int next = slice_of(0);
         for (int j0 = 0; j0 < nblk && ok; j0 += 16) {
           const int slices = next;
           if (j0 + 16 < nblk) next = slice_of(j0 + 16);
-          for (int j = j0; j < min(nblk, j0 + 16) && ok; ++j, ++g) {
+          const int j1 = min(nblk, j0 + 16);
+          for (int j = j0; j < j1 && ok; ++j, ++g) {
             const int s0 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0)), s1 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0) + 1);
             if (lane == 0) {
               const int st = g & 1;
               ok = mbar_wait(b_empty + 8 * st, ((g >> 1) & 1) ^ 1, abort_flag);
-              if (!ok) {
-                report(a.status, kErrProducer, 2 * g + (is_k ? 0 : 1));
-              } else {
+              if (ok) {
                 const uint32_t dst = s_dst + st * kTileBytes, bar = b_full + 8 * st;
                 mbar_arrive_expect_tx(bar, kTileBytes);
                 tma_load_3d(dst, tm, 0, 0, s0, bar);
@@ -386,18 +453,21 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tma_load_3d(dst + kBox, tm, 64, 0, s0, bar);
                 tma_load_3d(dst + kBox + kPageBox, tm, 64, 0, s1, bar);
                 ++issued;
+                if (!is_k && j >= check) mbar_arrive(b_look + 8 * st);   // PV(g-2) is done: v_full is at V(g)'s phase
               }
             }
             ok = __all_sync(0xffffffffu, ok);
           }
         }
+        if (!ok) break;
       }
       if (!ok && lane == 0) {
+        report(a.status, kErrProducer, 2 * g + (is_k ? 0 : 1));
         // Unwinding: let the copies already in flight land before the CTA's shared memory goes away.
         for (int spin = 0; spin < 100000; ++spin) {
           bool done = true;
-          for (int n = 0; n < 2; ++n) {
-            const int jg = issued - 1 - n, jq = q_issued - 1 - n;
+          for (int i = 1; i <= 2; ++i) {
+            const int jg = issued - i, jq = q_issued - i;
             if (jg >= 0) done = done && mbar_try_wait(b_full + 8 * (jg & 1), (jg >> 1) & 1);
             if (jq >= 0) done = done && mbar_try_wait(b_q_full + 8 * (jq & 1), (jq >> 1) & 1);
           }
@@ -409,7 +479,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     } else if (warp == 13) {
       // ================================ score-product issuer ==================================
       // A thread of its own for each of the two products: issuing one and testing barriers for the other in between
-      // does not keep the pipe fed.  S(g) goes into the buffer P(g-3) was read from: wait for that PV product first.
+      // does not keep the pipe fed.  S(g) goes into the buffer P(g-3) was read from: wait for that PV product first, and
+      // in a tile's third block also for the epilogue of the tile before, whose O that buffer takes over.
       if (lane == 0) {
         constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
         constexpr uint32_t idesc_qk = umma_idesc_f16(fmt, 0, kBM, kBN);
@@ -423,25 +494,36 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           dk_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sK + off, 16, 1024));
         }
         bool ok = true;
-        int g = 0;
+        int g = 0, freed = 0;                    // tiles whose O's region has been given back
+        int third[3] = {0, 0, 0};                // first block + 2 of the tiles freed + 1 .. (at most three are open)
+        uint32_t map = kRegions;
         for (int n = 0; ok; ++n) {
           const volatile Segment *seg = segment_at(n);
-          if (!seg) { report(a.status, kErrMma, -1000 - n); break; }
+          if (!seg) { ok = false; break; }
           if (!seg->more) break;
           const int nblk = seg->nblk;
+          if (n > 0) {
+            map = next_regions(map, g);
+            third[n % 3] = g + 2;
+          }
           ok = mbar_wait(b_q_full + 8 * (n & 1), (n >> 1) & 1, abort_flag);
-          if (!ok) { report(a.status, kErrMma, -1 - n); break; }
+          if (!ok) break;
           const uint32_t q_step = (n & 1) * kStageStep;
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = mbar_wait(b_k_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
-            if (!ok) { report(a.status, kErrMma, 4 * g); break; }
+            if (!ok) break;
+            if (freed < n && third[(freed + 1) % 3] == g) {
+              ok = mbar_wait(b_o_free + 8 * (freed & 3), (freed >> 2) & 1, abort_flag);
+              if (!ok) break;
+              ++freed;
+            }
             if (g >= kSBufs) {
               ok = mbar_wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1, abort_flag);
-              if (!ok) { report(a.status, kErrMma, 4 * g + 1); break; }
+              if (!ok) break;
             }
             tc_fence_after();
-            const uint32_t d_tmem = tmem + sb * 128, k_step = (g & 1) * kStageStep;
+            const uint32_t d_tmem = tmem + region(map, sb), k_step = (g & 1) * kStageStep;
 #pragma unroll
             for (int kk = 0; kk < kD / 16; ++kk) umma_ss_lo(d_tmem, dq_lo[kk] + q_step, dk_lo[kk] + k_step, d_hi, idesc_qk, kk > 0);
             umma_commit(b_s_full + 8 * sb);
@@ -449,6 +531,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           if (ok) umma_commit(b_q_empty + 8 * (n & 1));
         }
+        if (!ok) report(a.status, kErrMma, 2 * g);
       }
       __syncwarp();
     } else {
@@ -464,48 +547,129 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int kk = 0; kk < kBN / 16; ++kk) dv_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sV + kk * 2048, kBox, 1024));
         bool ok = true;
         int g = 0;
+        uint32_t looks = 0;                                  // bit st: parity of the looks at stage st so far
+        uint32_t map = kRegions;
         for (int n = 0; ok; ++n) {
           const volatile Segment *seg = segment_at(n);
-          if (!seg) { report(a.status, kErrMma, -1000 - n); break; }
+          if (!seg) { ok = false; break; }
           if (!seg->more) break;
-          const int nblk = seg->nblk;
+          const int nblk = seg->nblk, check = seg->check;
+          if (n > 0) map = next_regions(map, g);
+          const uint32_t o_tmem = tmem + region(map, 3);
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
-            if (!ok) { report(a.status, kErrMma, 4 * g + 2); break; }
-            if (j == 0 && n > 0) {   // the epilogue of the previous tile has read O
-              ok = mbar_wait(b_o_free, (n - 1) & 1, abort_flag);
-              if (!ok) { report(a.status, kErrMma, 4 * g + 3); break; }
+            if (!ok) break;
+            if (j == 0 && g > 0) {   // O goes where P(g-1) was
+              ok = mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag);
+              if (!ok) break;
+            }
+            if (j >= check) {
+              ok = mbar_wait(b_looked + 8 * (g & 1), (looks >> (g & 1)) & 1, abort_flag);
+              if (!ok) break;
+              looks ^= 1u << (g & 1);
             }
             ok = mbar_wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1, abort_flag);
-            if (!ok) { report(a.status, kErrMma, 4 * g + 3); break; }
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t p_tmem = tmem + sb * 128, v_step = (g & 1) * kStageStep;
+            const uint32_t p_tmem = tmem + region(map, sb), v_step = (g & 1) * kStageStep;
 #pragma unroll
             for (int kk = 0; kk < kBN / 16; ++kk)   // P: 16 packed 16-bit values = 8 TMEM columns per product
-              umma_ts_lo(tmem + kTmemO, p_tmem + kk * 8, dv_lo[kk] + v_step, d_hi, idesc_pv, (kk > 0 || j > 0) ? 1u : 0u);
+              umma_ts_lo(o_tmem, p_tmem + kk * 8, dv_lo[kk] + v_step, d_hi, idesc_pv, (kk > 0 || j > 0) ? 1u : 0u);
             umma_commit(b_pv_done + 8 * sb);
             umma_commit(b_v_empty + 8 * (g & 1));
-            if (j + 1 == nblk) umma_commit(b_o_full);
+            if (j + 1 == nblk) umma_commit(b_o_full + 8 * (n & 3));
           }
         }
+        if (!ok) report(a.status, kErrMma, 2 * g + 1);
       }
       __syncwarp();
     }
   } else if (warp >= 8) {
     // ================================ epilogue: O / l -> out, or (O, m, l) -> workspace ==========================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int r = (warp & 3) * 32 + lane;
-    const uint32_t tO = tmem + kTmemO + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-    const int tok = r / a.group, head = r % a.group;
-    for (int n = 0;; ++n) {
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const int tok = r / a.group;
+    // rows leave through a stage of 32 x 64 bytes per warp, four lanes to a row: whole sectors, eight rows to a store
+    unsigned char *const stage = smem + kOffStage + (warp & 3) * kStage;
+    int out_row[4];                                          // token << 8 | head
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (warp & 3) * 32 + 8 * i + (lane >> 2);
+      out_row[i] = (row / a.group) << 8 | (row % a.group);
+    }
+    uint32_t looks = 0, notes = 0, map = kRegions;
+    bool ok = true;
+    // A tile's first two blocks are looked through before the epilogue of the tile before, which their products do not
+    // wait for; its further blocks after it, because their scores do.
+    int g0 = 0, done = 0;                                    // first block of tile n, its blocks looked through
+    for (int n = 0; ok; ++n) {
       const volatile Segment *seg = segment_at(n);
-      if (!__all_sync(0xffffffffu, seg != nullptr)) { report(a.status, kErrEpilogue, -1000 - n); break; }
-      if (!seg->more) break;
+      ok = __all_sync(0xffffffffu, seg != nullptr);
+      if (!ok || !seg->more) break;
+      const int nblk = seg->nblk;
+      if (n > 0) map = next_regions(map, g0);
+      const volatile Segment *after = segment_at(n + 1);
+      ok = __all_sync(0xffffffffu, after != nullptr);
+      if (!ok) break;
+      const int early = after->more ? min(after->nblk, 2) : 0;
+      // ---- V rows that not every row of the tile sees; thread = row of V here ----
+      const int from = max(seg->check, done), turns = max(nblk - from, 0), after_from = early ? after->check : 0;
+      done = early;
+#pragma unroll 1
+      for (int i = 0; i < turns + max(early - after_from, 0); ++i) {
+        const bool here = i < turns;
+        const volatile Segment *of = here ? seg : after;
+        const int m = here ? n : n + 1, j = here ? from + i : after_from + i - turns;
+        const int g = (here ? g0 : g0 + nblk) + j, st = g & 1, col0 = (of->blk0 + j) * kBN;
+        const int lo = of->pos0 + 1 - col0, hi = of->len - col0;   // from lo on the first token sees nothing; the cache ends at hi
+        // the producer's word first: v_full alone tells two phases apart, not three
+        ok = mbar_wait(b_look + 8 * st, (looks >> st) & 1, abort_flag) && mbar_wait(b_v_full + 8 * st, (g >> 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        looks ^= 1u << st;
+        unsigned char *row = smem + (4 + st) * kTileBytes + r * 128;
+        if (r >= hi) {
+#pragma unroll 4
+          for (int c = 0; c < 16; ++c)
+            *reinterpret_cast<uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        } else if (r >= lo) {
+          uint32_t probe[4] = {0u, 0u, 0u, 0u};
+#pragma unroll 4
+          for (int c = 0; c < 16; ++c) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16);
+            probe[0] = finite_probe<DT>(x.x, probe[0]);
+            probe[1] = finite_probe<DT>(x.y, probe[1]);
+            probe[2] = finite_probe<DT>(x.z, probe[2]);
+            probe[3] = finite_probe<DT>(x.w, probe[3]);
+          }
+          bool clean = true;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) clean = clean && !not_finite16<DT>(probe[c] & 0xffffu) && !not_finite16<DT>(probe[c] >> 16);
+          if (!clean) {
+#pragma unroll 1
+            for (int c = 0; c < kD; ++c) {   // column c: 16-byte piece (c / 8) % 8 of its half, swizzled with the row
+              uint16_t *x = reinterpret_cast<uint16_t *>(row + (c >> 6) * kBox + (((c >> 3) ^ r) & 7) * 16) + (c & 7);
+              if (not_finite16<DT>(*x)) {
+                *x = 0;
+                atomicMax(&sh->taint[m & 1][c], (static_cast<unsigned long long>(m + 1) << 32) | (0x7fffffffu - static_cast<unsigned>(col0 + r)));
+                *reinterpret_cast<volatile int *>(&sh->taint_any[m & 1]) = m + 1;
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(b_looked + 8 * st);
+        __syncwarp();
+      }
+      if (!ok) break;
+      g0 += nblk;
       const int slot = seg->slot;
-      const bool row_exists = tok < seg->ntok;
+      const int ntok = seg->ntok;
       const int last_seen = min(seg->pos0 + tok, seg->len - 1);
-      uint16_t *dst = a.out + static_cast<long long>(seg->tok0 + tok) * a.out_t + static_cast<long long>(seg->kvh * a.group + head) * a.out_h;
+      uint16_t *const dst = a.out + seg->tok0 * a.out_t + static_cast<long long>(seg->kvh) * a.group * a.out_h + (lane & 3) * 8;
+      const uint32_t tO = tmem + region(map, 3) + lane_addr;
       // a table entry outside the pool among the pages read: NaN instead of a sum that lacks them
       bool bad = false;
       {
@@ -514,86 +678,102 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         for (int p = 2 * seg->blk0 + lane; p < end; p += 32) bad = bad || static_cast<unsigned>(table[p]) >= static_cast<unsigned>(a.num_pages);
         bad = __any_sync(0xffffffffu, bad);
       }
-      bool ok = __all_sync(0xffffffffu, mbar_wait(b_lm_ready, n & 1, abort_flag));
-      if (!ok) { report(a.status, kErrEpilogue, 2 * n); break; }
-      const float m0 = sh->lm[0][r][0], l0 = sh->lm[0][r][1], m1 = sh->lm[1][r][0], l1 = sh->lm[1][r][1];
-      const bool tainted = *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) == n + 1;
-      if (!tainted) mbar_arrive(b_lm_free);   // else the notes of this tile are still to be read
-      const float mf = fmaxf(m0, m1);         // the running maximum never decreases: the later one is the larger
-      float l = (l0 == 0.f ? 0.f : l0 * ex2(m0 - mf)) + (l1 == 0.f ? 0.f : l1 * ex2(m1 - mf));
-      const bool empty = l == 0.f;            // no visible row (in this part): 0, whatever the products hold
+      ok = __all_sync(0xffffffffu, mbar_wait(b_lm_ready + 8 * (n & 1), (n >> 1) & 1, abort_flag));
+      if (!ok) break;
+      const float2 lm0 = sh->lm[n & 1][0][r], lm1 = sh->lm[n & 1][1][r];
+      mbar_arrive(b_lm_free + 8 * (n & 1));
+      const float mf = fmaxf(lm0.x, lm1.x);   // the running maximum never decreases: the later one is the larger
+      float l = (lm0.y == 0.f ? 0.f : lm0.y * ex2(lm0.x - mf)) + (lm1.y == 0.f ? 0.f : lm1.y * ex2(lm1.x - mf));
+      // no visible row (in this part): every weight was 0 and every V looked through, so O is 0
+      const bool empty = l == 0.f;
       if (bad) l = __int_as_float(0x7fffffff);
-      const float inv = empty && !bad ? 0.f : (slot < 0 ? 1.f / l : 1.f);
+      const float inv = slot >= 0 || (empty && !bad) ? 1.f : 1.f / l;
+      const uint64_t inv2 = f2_pack(inv, inv);
       float *po = nullptr;
       if (slot >= 0) {
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + r;
-        po = a.part_o + pr * kD;
-        if (row_exists) a.part_ml[pr] = make_float2(mf, l);
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + (warp & 3) * 32;
+        po = a.part_o + (pr + lane) * kD;
+        if (tok < ntok) a.part_ml[pr + lane] = make_float2(mf, l);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(b_o_full, n & 1, abort_flag));
-      if (!ok) { report(a.status, kErrEpilogue, 2 * n + 1); break; }
+      ok = __all_sync(0xffffffffu, mbar_wait(b_o_full + 8 * (n & 3), (n >> 2) & 1, abort_flag));
+      if (!ok) break;
       tc_fence_after();
+      // the PV products waited for every look at the tile's V, so the notes of all the warps are there
+      const bool tainted = *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) == n + 1;
+      auto noted = [&](int c) -> bool {       // column c of this row holds a value that is not finite
+        const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
+        return static_cast<int>(note >> 32) == n + 1 && static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) <= last_seen;
+      };
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];
         tmem_ld32(tO + c * 32, o);
         tmem_wait_ld();
-        if (c == kD / 32 - 1) {   // O is in registers: the next tile may overwrite it
+        if (c == kD / 32 - 1) {   // O is in registers: its region may be overwritten
           tc_fence_before();
-          mbar_arrive(b_o_free);
+          mbar_arrive(b_o_free + 8 * (n & 3));
         }
+        if (slot < 0) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[k]) * inv);
-        if (tainted) {
-#pragma unroll 1
-          for (int k = 0; k < 32; ++k) {
-            const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c * 32 + k]);
-            if (static_cast<int>(note >> 32) == n + 1 && static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) <= last_seen) {
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (i == k) o[i] = 0x7fffffffu;
+            for (int i = 0; i < 4; ++i) {
+              const float2 x = f2_unpack(f2_mul(f2_pack(__uint_as_float(o[8 * k + 2 * i]), __uint_as_float(o[8 * k + 2 * i + 1])), inv2));
+              w[i] = pack2<DT>(x.x, x.y);
             }
+            *reinterpret_cast<uint4 *>(stage + lane * 64 + ((k ^ (lane >> 1)) & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-        }
-        if (row_exists) {
-          if (slot < 0) {
+          if (tainted) {
+#pragma unroll 1
+            for (int k = 0; k < 32; ++k)
+              if (noted(c * 32 + k)) *reinterpret_cast<uint16_t *>(stage + lane * 64 + (((k >> 3) ^ (lane >> 1)) & 3) * 16 + (k & 7) * 2) = 0x7fffu;
+          }
+          __syncwarp();
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              uint4 w;
-              w.x = pack2<DT>(__uint_as_float(o[8 * k + 0]), __uint_as_float(o[8 * k + 1]));
-              w.y = pack2<DT>(__uint_as_float(o[8 * k + 2]), __uint_as_float(o[8 * k + 3]));
-              w.z = pack2<DT>(__uint_as_float(o[8 * k + 4]), __uint_as_float(o[8 * k + 5]));
-              w.w = pack2<DT>(__uint_as_float(o[8 * k + 6]), __uint_as_float(o[8 * k + 7]));
-              *reinterpret_cast<uint4 *>(dst + c * 32 + k * 8) = w;
-            }
-          } else {
+          for (int i = 0; i < 4; ++i) {
+            const int row = 8 * i + (lane >> 2);
+            const uint4 x = *reinterpret_cast<const uint4 *>(stage + row * 64 + ((lane ^ (row >> 1)) & 3) * 16);
+            if ((out_row[i] >> 8) < ntok)
+              *reinterpret_cast<uint4 *>(dst + (out_row[i] >> 8) * a.out_t + (out_row[i] & 0xff) * a.out_h + c * 32) = x;
+          }
+          __syncwarp();
+        } else {   // twice per CTA at most: straight from the registers
+          if (tok < ntok) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              reinterpret_cast<uint4 *>(po + c * 32)[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              *reinterpret_cast<uint4 *>(po + c * 32 + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            if (tainted) {
+#pragma unroll 1
+              for (int k = 0; k < 32; ++k)
+                if (noted(c * 32 + k)) po[c * 32 + k] = __int_as_float(0x7fffffff);
+            }
           }
+          __syncwarp();
         }
-        __syncwarp();   // the next load from TMEM is one for the whole warp
       }
-      if (tainted) mbar_arrive(b_lm_free);
+      if (tainted) {   // every warp has read its notes before any looks on and writes over them
+        mbar_arrive(b_notes_read);
+        ok = __all_sync(0xffffffffu, mbar_wait(b_notes_read, notes, abort_flag));
+        notes ^= 1;
+      }
     }
+    if (!ok && lane == 0) report(a.status, kErrEpilogue, g0);
   } else {
     // ================================ softmax: warpgroup w takes the blocks g with g & 1 == w ================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
     const int w = warp >> 2;
     const int r = (warp & 3) * 32 + lane;                     // row in the tile == TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + kTmemO + lane_addr;
     const int tok = r / a.group;
     int n = 0, g0 = 0;
+    uint32_t map = kRegions;
     bool ok = true, more = true;
     int nblk = 0, blk0 = 0, pos0 = 0, len = 0, ntok = 0;
     auto read_segment = [&]() {
       const volatile Segment *seg = segment_at(n);
       ok = __all_sync(0xffffffffu, seg != nullptr);
-      if (!ok) {
-        report(a.status, kErrSoftmax, -1000 - n);
-        return;
-      }
+      if (!ok) return;
       more = seg->more;
       nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
     };
@@ -602,17 +782,17 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int g = w; ok; g += 2) {
       // tiles that end before block g: hand (maximum, partial sum) to the epilogue and move on
       while (more && g >= g0 + nblk) {
-        if (n > 0) {   // the epilogue has read the previous tile's values
-          ok = __all_sync(0xffffffffu, mbar_wait(b_lm_free, (n - 1) & 1, abort_flag));
-          if (!ok) { report(a.status, kErrSoftmax, -1 - n); break; }
+        if (n > 1) {   // the epilogue has read the values of the tile before the previous one
+          ok = __all_sync(0xffffffffu, mbar_wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag));
+          if (!ok) break;
         }
-        sh->lm[w][r][0] = m_mine;
-        sh->lm[w][r][1] = l;
-        mbar_arrive(b_lm_ready);
+        sh->lm[n & 1][w][r] = make_float2(m_mine, l);
+        mbar_arrive(b_lm_ready + 8 * (n & 1));
         m_mine = -INFINITY;
         l = 0.f;
         g0 += nblk;
         ++n;
+        map = next_regions(map, g0);
         read_segment();
         if (!ok) break;
       }
@@ -620,15 +800,15 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int j = g - g0;
       const int sb = g % kSBufs;
       const int col0 = (blk0 + j) * kBN;                       // cache row of the block's first column
-      const uint32_t tS = tmem + sb * 128 + lane_addr;
+      const uint32_t tS = tmem + region(map, sb) + lane_addr;
       ok = __all_sync(0xffffffffu, mbar_wait(b_s_full + 8 * sb, (g / kSBufs) & 1, abort_flag));
-      if (!ok) { report(a.status, kErrSoftmax, g); break; }
+      if (!ok) break;
       tc_fence_after();
       float m_prev = -INFINITY;
       if (g > 0) {
         // block g-1 has decided on its maximum (and, before that, has read the slot this block will overwrite)
         ok = __all_sync(0xffffffffu, mbar_wait(b_m_ready + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag));
-        if (!ok) { report(a.status, kErrSoftmax, 1000 + g); break; }
+        if (!ok) break;
         if (j > 0) m_prev = sh->mslot[(g - 1) & 1][r];
       }
       // column c of the block is seen by this row iff c <= vis
@@ -676,9 +856,10 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (__any_sync(0xffffffffu, need)) {
           // O must hold every product up to block g-1 and none may be in flight
           ok = __all_sync(0xffffffffu, mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag));
-          if (!ok) { report(a.status, kErrSoftmax, 2000 + g); break; }
+          if (!ok) break;
           tc_fence_after();
           const float f = need ? ex2(m_prev - m_blk) : 1.f;
+          const uint32_t tO = tmem + region(map, 3) + lane_addr;
 #pragma unroll 1
           for (int c = 0; c < kD / 16; ++c) {
             uint32_t o[16];
@@ -715,47 +896,11 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const float2 ls = f2_unpack(lsum2);
         l += ls.x + ls.y;
       }
-      // ---- V rows that not every row of the tile sees ----
-      const int lo = max(pos0 + 1 - col0, 0), hi = max(len - col0, 0);   // from lo on the first token sees nothing; the cache ends at hi
-      if (min(lo, hi) < kBN) {
-        // V(g-2), in the same buffer, must have come and gone first: the barrier tells two phases apart, not three
-        if (g >= 2) ok = mbar_wait(b_pv_done + 8 * ((g - 2) % kSBufs), ((g - 2) / kSBufs) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok && mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag));
-        if (!ok) { report(a.status, kErrSoftmax, 3000 + g); break; }
-        unsigned char *row = smem + 4 * kTileBytes + (g & 1) * kTileBytes + r * 128;   // thread = row of V here
-        if (r >= hi) {
-#pragma unroll
-          for (int c = 0; c < 16; ++c)
-            *reinterpret_cast<uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        } else if (r >= lo) {
-          uint32_t probe = 0u;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(row + (c >> 3) * kBox + ((c + r) & 7) * 16);
-            probe = finite_probe<DT>(x.x, probe);
-            probe = finite_probe<DT>(x.y, probe);
-            probe = finite_probe<DT>(x.z, probe);
-            probe = finite_probe<DT>(x.w, probe);
-          }
-          if (not_finite16<DT>(probe & 0xffffu) || not_finite16<DT>(probe >> 16)) {
-#pragma unroll 1
-            for (int c = 0; c < kD; ++c) {   // column c: 16-byte piece (c / 8) % 8 of its half, swizzled with the row
-              uint16_t *x = reinterpret_cast<uint16_t *>(row + (c >> 6) * kBox + (((c >> 3) ^ r) & 7) * 16) + (c & 7);
-              if (not_finite16<DT>(*x)) {
-                *x = 0;
-                atomicMax(&sh->taint[n & 1][c], (static_cast<unsigned long long>(n + 1) << 32) | (0x7fffffffu - static_cast<unsigned>(col0 + r)));
-                *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) = n + 1;
-              }
-            }
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive(b_p_full + 8 * sb);
     }
+    if (!ok && lane == 0) report(a.status, kErrSoftmax, g0);
   }
 
   // ================================ tear-down =====================================
@@ -875,6 +1020,11 @@ extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *
   NB200_REQUIRE(Hq <= 65535, NB200_ERR_UNSUPPORTED, "%s: too many heads", who);
   NB200_REQUIRE(T < (1 << 30) && max_pages <= (1 << 30) / kPageRows, NB200_ERR_UNSUPPORTED,
                 "%s: T or max_pages * page_size does not fit 30 bits", who);
+  // the device counts blocks in 32 bits: tiles (their number bounded by full tiles and one remainder per sequence) times
+  // the longest sequence's blocks
+  const double tiles = (static_cast<double>(T) / (kBM / (Hq / Hkv)) + B) * Hkv;
+  NB200_REQUIRE(tiles * (max_pages / 2 + 2.0 + kTileUnits) < 4.0e9, NB200_ERR_UNSUPPORTED,
+                "%s: T and max_pages are too large for one call", who);
   NB200_REQUIRE(static_cast<long long>(num_pages) * Hkv < (1ll << 31) - 1, NB200_ERR_UNSUPPORTED,
                 "%s: num_pages * Hkv does not fit 31 bits", who);
   NB200_REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace),
