@@ -42,7 +42,7 @@
 // replaced by 0 and noted; the epilogue makes it a NaN in exactly those rows that see it.  Done by the softmax warps, the
 // same look cost 44 of 211 us at a 4096-token first chunk.
 //
-// Every wait is bounded; on expiry the CTA records a code in the status words and unwinds.
+// Every wait is bounded; on expiry the role records a code in the status words and unwinds.
 #include <cuda.h>
 
 #include <atomic>
@@ -92,8 +92,8 @@ struct Owner {
 };
 struct Args {
   const int *block_table, *cu_seqlens, *seq_lens;
-  uint16_t *out;
-  long long out_t, out_h;
+  uint4 *out;
+  unsigned out_t, out_h;     // in 16 bytes
   int T, B, Hkv, group, tok_tile, num_pages, max_pages;
   float scale_log2;
   float *part_o;             // [kMaxCtas][2][128][128]
@@ -117,7 +117,6 @@ struct Shared {
   int start_b;
   int taint_any[2];                  // tile number + 1
   uint32_t tmem_base;
-  int abort_flag;
   int skip;
   float mslot[2][kBM];               // running maximum decided by block g, slot g & 1
   float2 lm[2][2][kBM];              // of tile n in [n & 1], per warpgroup: (maximum last used, partial row sum)
@@ -133,6 +132,24 @@ __device__ __forceinline__ void report(int *status, int code, int detail) {
     status[2] = detail;
     status[3] = static_cast<int>(threadIdx.x);
   }
+}
+
+// Waits for a phase with a limit on the turns: about 2 s if every turn suspends the thread for its microsecond, at least
+// 0.1 s.  A role whose wait runs out leaves, and the waits of the others then run out too.  Less code than a clock and
+// a flag to look at, and code is what this kernel is short of: its roles' paths at a change of tiles share the
+// instruction cache (117 KB of it took 221 us at a 4096-token first chunk, 86 KB 185 us).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 2000000; ++i)
+    if (mbar_try_wait_suspend(bar, parity, 1000u)) return true;
+  return false;
+}
+// The same without suspending (test_wait): the waiter goes on a few cycles after the phase completes.  For an issuing thread.
+__device__ __forceinline__ bool wait_poll(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 1 << 26; ++i)
+    if (mbar_test_wait(bar, parity)) return true;
+  return false;
 }
 
 // New tokens of a sequence, where they sit and what there is to see.  Clamped, so that no device-side value leads out of
@@ -206,7 +223,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   const uint32_t sK = base + 2 * kTileBytes;                  // stage g & 1
   const uint32_t sV = base + 4 * kTileBytes;
   Shared *sh = reinterpret_cast<Shared *>(smem + kOffShared);
-  volatile int *abort_flag = &sh->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
@@ -219,7 +235,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
-    sh->abort_flag = 0;
     sh->start_b = 0;
     sh->before = 0;
     sh->taint_any[0] = sh->taint_any[1] = 0;
@@ -315,7 +330,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   // apart (two Q buffers, two stages, three score buffers, O's of three tiles), so 16 slots need no "empty" barrier.
   // Null: an expired wait.
   auto segment_at = [&](int n) -> const volatile Segment * {
-    if (!mbar_wait(b_sched + 8 * (n % kSched), (n / kSched) & 1, abort_flag)) return nullptr;
+    if (!wait(b_sched + 8 * (n % kSched), (n / kSched) & 1)) return nullptr;
     return &sh->seg[n % kSched];
   };
 
@@ -426,7 +441,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
         int next = slice_of(0);
         if (is_k && lane == 0) {
-          ok = mbar_wait(b_q_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag);
+          ok = wait(b_q_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1);
           if (ok) {
             const int tok0 = seg->tok0;
             mbar_arrive_expect_tx(b_q_full + 8 * (n & 1), q_bytes);
@@ -444,7 +459,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             const int s0 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0)), s1 = __shfl_sync(0xffffffffu, slices, 2 * (j - j0) + 1);
             if (lane == 0) {
               const int st = g & 1;
-              ok = mbar_wait(b_empty + 8 * st, ((g >> 1) & 1) ^ 1, abort_flag);
+              ok = wait(b_empty + 8 * st, ((g >> 1) & 1) ^ 1);
               if (ok) {
                 const uint32_t dst = s_dst + st * kTileBytes, bar = b_full + 8 * st;
                 mbar_arrive_expect_tx(bar, kTileBytes);
@@ -506,20 +521,20 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             map = next_regions(map, g);
             third[n % 3] = g + 2;
           }
-          ok = mbar_wait(b_q_full + 8 * (n & 1), (n >> 1) & 1, abort_flag);
+          ok = wait(b_q_full + 8 * (n & 1), (n >> 1) & 1);
           if (!ok) break;
           const uint32_t q_step = (n & 1) * kStageStep;
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
-            ok = mbar_wait(b_k_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
+            ok = wait(b_k_full + 8 * (g & 1), (g >> 1) & 1);
             if (!ok) break;
             if (freed < n && third[(freed + 1) % 3] == g) {
-              ok = mbar_wait(b_o_free + 8 * (freed & 3), (freed >> 2) & 1, abort_flag);
+              ok = wait(b_o_free + 8 * (freed & 3), (freed >> 2) & 1);
               if (!ok) break;
               ++freed;
             }
             if (g >= kSBufs) {
-              ok = mbar_wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1, abort_flag);
+              ok = wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1);
               if (!ok) break;
             }
             tc_fence_after();
@@ -558,18 +573,18 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const uint32_t o_tmem = tmem + region(map, 3);
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
-            ok = mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
+            ok = wait(b_v_full + 8 * (g & 1), (g >> 1) & 1);
             if (!ok) break;
             if (j == 0 && g > 0) {   // O goes where P(g-1) was
-              ok = mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag);
+              ok = wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1);
               if (!ok) break;
             }
             if (j >= check) {
-              ok = mbar_wait(b_looked + 8 * (g & 1), (looks >> (g & 1)) & 1, abort_flag);
+              ok = wait(b_looked + 8 * (g & 1), (looks >> (g & 1)) & 1);
               if (!ok) break;
               looks ^= 1u << (g & 1);
             }
-            ok = mbar_wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1, abort_flag);
+            ok = wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1);
             if (!ok) break;
             tc_fence_after();
             const uint32_t p_tmem = tmem + region(map, sb), v_step = (g & 1) * kStageStep;
@@ -625,7 +640,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const int g = (here ? g0 : g0 + nblk) + j, st = g & 1, col0 = (of->blk0 + j) * kBN;
         const int lo = of->pos0 + 1 - col0, hi = of->len - col0;   // from lo on the first token sees nothing; the cache ends at hi
         // the producer's word first: v_full alone tells two phases apart, not three
-        ok = mbar_wait(b_look + 8 * st, (looks >> st) & 1, abort_flag) && mbar_wait(b_v_full + 8 * st, (g >> 1) & 1, abort_flag);
+        ok = wait(b_look + 8 * st, (looks >> st) & 1) && wait(b_v_full + 8 * st, (g >> 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         looks ^= 1u << st;
@@ -668,17 +683,18 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int slot = seg->slot;
       const int ntok = seg->ntok;
       const int last_seen = min(seg->pos0 + tok, seg->len - 1);
-      uint16_t *const dst = a.out + seg->tok0 * a.out_t + static_cast<long long>(seg->kvh) * a.group * a.out_h + (lane & 3) * 8;
+      uint4 *const dst = a.out + static_cast<size_t>(seg->tok0) * a.out_t + static_cast<size_t>(seg->kvh * a.group) * a.out_h;
       const uint32_t tO = tmem + region(map, 3) + lane_addr;
       // a table entry outside the pool among the pages read: NaN instead of a sum that lacks them
       bool bad = false;
       {
         const int *table = a.block_table + static_cast<long long>(seg->b) * a.max_pages;
         const int end = min(2 * (seg->blk0 + seg->nblk), (seg->len + kPageRows - 1) / kPageRows);
+#pragma unroll 1
         for (int p = 2 * seg->blk0 + lane; p < end; p += 32) bad = bad || static_cast<unsigned>(table[p]) >= static_cast<unsigned>(a.num_pages);
         bad = __any_sync(0xffffffffu, bad);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(b_lm_ready + 8 * (n & 1), (n >> 1) & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, wait(b_lm_ready + 8 * (n & 1), (n >> 1) & 1));
       if (!ok) break;
       const float2 lm0 = sh->lm[n & 1][0][r], lm1 = sh->lm[n & 1][1][r];
       mbar_arrive(b_lm_free + 8 * (n & 1));
@@ -695,15 +711,11 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         po = a.part_o + (pr + lane) * kD;
         if (tok < ntok) a.part_ml[pr + lane] = make_float2(mf, l);
       }
-      ok = __all_sync(0xffffffffu, mbar_wait(b_o_full + 8 * (n & 3), (n >> 2) & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, wait(b_o_full + 8 * (n & 3), (n >> 2) & 1));
       if (!ok) break;
       tc_fence_after();
       // the PV products waited for every look at the tile's V, so the notes of all the warps are there
       const bool tainted = *reinterpret_cast<volatile int *>(&sh->taint_any[n & 1]) == n + 1;
-      auto noted = [&](int c) -> bool {       // column c of this row holds a value that is not finite
-        const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
-        return static_cast<int>(note >> 32) == n + 1 && static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) <= last_seen;
-      };
 #pragma unroll 1
       for (int c = 0; c < kD / 32; ++c) {
         uint32_t o[32];
@@ -724,18 +736,13 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             }
             *reinterpret_cast<uint4 *>(stage + lane * 64 + ((k ^ (lane >> 1)) & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
           }
-          if (tainted) {
-#pragma unroll 1
-            for (int k = 0; k < 32; ++k)
-              if (noted(c * 32 + k)) *reinterpret_cast<uint16_t *>(stage + lane * 64 + (((k >> 3) ^ (lane >> 1)) & 3) * 16 + (k & 7) * 2) = 0x7fffu;
-          }
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = 8 * i + (lane >> 2);
             const uint4 x = *reinterpret_cast<const uint4 *>(stage + row * 64 + ((lane ^ (row >> 1)) & 3) * 16);
             if ((out_row[i] >> 8) < ntok)
-              *reinterpret_cast<uint4 *>(dst + (out_row[i] >> 8) * a.out_t + (out_row[i] & 0xff) * a.out_h + c * 32) = x;
+              dst[static_cast<size_t>(out_row[i] >> 8) * a.out_t + static_cast<size_t>(out_row[i] & 0xff) * a.out_h + c * 4 + (lane & 3)] = x;
           }
           __syncwarp();
         } else {   // twice per CTA at most: straight from the registers
@@ -743,18 +750,26 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
             for (int k = 0; k < 8; ++k)
               *reinterpret_cast<uint4 *>(po + c * 32 + 4 * k) = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-            if (tainted) {
-#pragma unroll 1
-              for (int k = 0; k < 32; ++k)
-                if (noted(c * 32 + k)) po[c * 32 + k] = __int_as_float(0x7fffffff);
-            }
           }
           __syncwarp();
         }
       }
-      if (tainted) {   // every warp has read its notes before any looks on and writes over them
+      if (tainted) {   // columns whose values are not finite: NaN in the rows that see them
+        __syncwarp();
+        uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(r % a.group) * a.out_h);
+#pragma unroll 1
+        for (int c = 0; c < kD && tok < ntok; ++c) {
+          const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
+          if (static_cast<int>(note >> 32) != n + 1 || static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) > last_seen) continue;
+          if (slot < 0)
+            mine[c] = 0x7fffu;
+          else
+            po[c] = __int_as_float(0x7fffffff);
+        }
+        __syncwarp();
+        // every warp has read its notes before any looks on and writes over them
         mbar_arrive(b_notes_read);
-        ok = __all_sync(0xffffffffu, mbar_wait(b_notes_read, notes, abort_flag));
+        ok = __all_sync(0xffffffffu, wait(b_notes_read, notes));
         notes ^= 1;
       }
     }
@@ -783,7 +798,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // tiles that end before block g: hand (maximum, partial sum) to the epilogue and move on
       while (more && g >= g0 + nblk) {
         if (n > 1) {   // the epilogue has read the values of the tile before the previous one
-          ok = __all_sync(0xffffffffu, mbar_wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag));
+          ok = __all_sync(0xffffffffu, wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1));
           if (!ok) break;
         }
         sh->lm[n & 1][w][r] = make_float2(m_mine, l);
@@ -801,13 +816,13 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int sb = g % kSBufs;
       const int col0 = (blk0 + j) * kBN;                       // cache row of the block's first column
       const uint32_t tS = tmem + region(map, sb) + lane_addr;
-      ok = __all_sync(0xffffffffu, mbar_wait(b_s_full + 8 * sb, (g / kSBufs) & 1, abort_flag));
+      ok = __all_sync(0xffffffffu, wait(b_s_full + 8 * sb, (g / kSBufs) & 1));
       if (!ok) break;
       tc_fence_after();
       float m_prev = -INFINITY;
       if (g > 0) {
         // block g-1 has decided on its maximum (and, before that, has read the slot this block will overwrite)
-        ok = __all_sync(0xffffffffu, mbar_wait(b_m_ready + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag));
+        ok = __all_sync(0xffffffffu, wait(b_m_ready + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1));
         if (!ok) break;
         if (j > 0) m_prev = sh->mslot[(g - 1) & 1][r];
       }
@@ -855,7 +870,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         mbar_arrive(b_m_ready + 8 * (g & 1));
         if (__any_sync(0xffffffffu, need)) {
           // O must hold every product up to block g-1 and none may be in flight
-          ok = __all_sync(0xffffffffu, mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag));
+          ok = __all_sync(0xffffffffu, wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1));
           if (!ok) break;
           tc_fence_after();
           const float f = need ? ex2(m_prev - m_blk) : 1.f;
@@ -946,7 +961,7 @@ template <int DT> __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t *dst = a.out + static_cast<long long>(own.tok0 + r / a.group) * a.out_t + static_cast<long long>(own.kvh * a.group + r % a.group) * a.out_h;
+  uint4 *dst = a.out + static_cast<size_t>(own.tok0 + r / a.group) * a.out_t + static_cast<size_t>(own.kvh * a.group + r % a.group) * a.out_h;
   reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
 }
 
@@ -1033,12 +1048,12 @@ extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *
   long long s[4];
   for (int i = 0; i < 4; ++i) {
     s[i] = extents[i] == 1 ? kD : strides[i];              // a stride that is never taken
-    NB200_REQUIRE(s[i] >= kD && s[i] % 8 == 0 && s[i] < (1ll << 38), NB200_ERR_BAD_ARG,
+    NB200_REQUIRE(s[i] >= kD && s[i] % 8 == 0 && s[i] < (1ll << 34), NB200_ERR_BAD_ARG,
                   "%s: the strides of q and out must be multiples of 16 bytes, at least a row", who);
   }
   Args a{};
   a.block_table = block_table, a.cu_seqlens = cu_seqlens, a.seq_lens = seq_lens;
-  a.out = static_cast<uint16_t *>(out), a.out_t = s[2], a.out_h = s[3];
+  a.out = static_cast<uint4 *>(out), a.out_t = static_cast<unsigned>(s[2] / 8), a.out_h = static_cast<unsigned>(s[3] / 8);
   a.T = T, a.B = B, a.Hkv = Hkv, a.group = Hq / Hkv, a.tok_tile = kBM / a.group;
   a.num_pages = num_pages, a.max_pages = max_pages, a.scale_log2 = scale_log2, a.status = status;
   char *ws = static_cast<char *>(workspace);
