@@ -70,7 +70,7 @@ constexpr int kTmemCols = 512;                  // four regions of 128 columns
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kSched = 16;                      // ring of tile descriptors handed from the K producer to the other roles
 constexpr int kMaxCtas = 160;                   // CTAs that the workspace has room for
-constexpr int kTileUnits = 1;                   // what changing tiles costs, in blocks, on the line that is cut
+constexpr int kTileUnits = 2;                   // what changing tiles costs (2 us), in blocks, on the line that is cut
 
 enum : int { kErrProducer = 41, kErrMma = 42, kErrSoftmax = 43, kErrEpilogue = 44, kErrTable = 22, kErrSlot = 23 };
 
@@ -500,14 +500,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
         constexpr uint32_t idesc_qk = umma_idesc_f16(fmt, 0, kBM, kBN);
         const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
-        uint32_t dq_lo[kD / 16], dk_lo[kD / 16];   // buffer / stage 1 is kStageStep further
-        constexpr uint32_t kStageStep = kTileBytes >> 4;
-#pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32;
-          dq_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sQ + off, 16, 1024));
-          dk_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sK + off, 16, 1024));
-        }
+        const uint32_t dq = static_cast<uint32_t>(umma_desc_sw128(sQ, 16, 1024)), dk = static_cast<uint32_t>(umma_desc_sw128(sK, 16, 1024));
+        constexpr uint32_t kStageStep = kTileBytes >> 4;   // of buffer / stage 1
         bool ok = true;
         int g = 0, freed = 0;                    // tiles whose O's region has been given back
         int third[3] = {0, 0, 0};                // first block + 2 of the tiles freed + 1 .. (at most three are open)
@@ -538,9 +532,13 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               if (!ok) break;
             }
             tc_fence_after();
-            const uint32_t d_tmem = tmem + region(map, sb), k_step = (g & 1) * kStageStep;
+            const uint32_t d_tmem = tmem + region(map, sb);
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {          // 64 columns each: 16 of them are 32 bytes of a swizzled row
+              const uint32_t q_at = dq + q_step + half * (kBox >> 4), k_at = dk + (g & 1) * kStageStep + half * (kBox >> 4);
 #pragma unroll
-            for (int kk = 0; kk < kD / 16; ++kk) umma_ss_lo(d_tmem, dq_lo[kk] + q_step, dk_lo[kk] + k_step, d_hi, idesc_qk, kk > 0);
+              for (int kk = 0; kk < 4; ++kk) umma_ss_lo(d_tmem, q_at + kk * 2, k_at + kk * 2, d_hi, idesc_qk, half | kk);
+            }
             umma_commit(b_s_full + 8 * sb);
             umma_commit(b_k_empty + 8 * (g & 1));
           }
@@ -556,10 +554,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         constexpr uint32_t idesc_pv = umma_idesc_f16(fmt, 1, kBM, kD);
         // V is MN-major: 16 kv rows = 2 KB, the two 64-column halves kBox apart
         const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
-        uint32_t dv_lo[kBN / 16];
+        const uint32_t dv = static_cast<uint32_t>(umma_desc_sw128(sV, kBox, 1024));
         constexpr uint32_t kStageStep = kTileBytes >> 4;
-#pragma unroll
-        for (int kk = 0; kk < kBN / 16; ++kk) dv_lo[kk] = static_cast<uint32_t>(umma_desc_sw128(sV + kk * 2048, kBox, 1024));
         bool ok = true;
         int g = 0;
         uint32_t looks = 0;                                  // bit st: parity of the looks at stage st so far
@@ -587,10 +583,13 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             ok = wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t p_tmem = tmem + region(map, sb), v_step = (g & 1) * kStageStep;
+            const uint32_t p_tmem = tmem + region(map, sb), v_at = dv + (g & 1) * kStageStep;
+#pragma unroll 1
+            for (int k0 = 0; k0 < kBN / 16; k0 += 4) {
 #pragma unroll
-            for (int kk = 0; kk < kBN / 16; ++kk)   // P: 16 packed 16-bit values = 8 TMEM columns per product
-              umma_ts_lo(o_tmem, p_tmem + kk * 8, dv_lo[kk] + v_step, d_hi, idesc_pv, (kk > 0 || j > 0) ? 1u : 0u);
+              for (int kk = 0; kk < 4; ++kk)   // P: 16 packed 16-bit values = 8 TMEM columns per product
+                umma_ts_lo(o_tmem, p_tmem + (k0 + kk) * 8, v_at + (k0 + kk) * 128, d_hi, idesc_pv, k0 | kk | j);
+            }
             umma_commit(b_pv_done + 8 * sb);
             umma_commit(b_v_empty + 8 * (g & 1));
             if (j + 1 == nblk) umma_commit(b_o_full + 8 * (n & 3));
@@ -781,35 +780,28 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int r = (warp & 3) * 32 + lane;                     // row in the tile == TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int tok = r / a.group;
-    int n = 0, g0 = 0;
+    int n = -1, g0 = 0;
     uint32_t map = kRegions;
     bool ok = true, more = true;
     int nblk = 0, blk0 = 0, pos0 = 0, len = 0, ntok = 0;
-    auto read_segment = [&]() {
-      const volatile Segment *seg = segment_at(n);
-      ok = __all_sync(0xffffffffu, seg != nullptr);
-      if (!ok) return;
-      more = seg->more;
-      nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
-    };
-    read_segment();
     float m_mine = -INFINITY, l = 0.f;
     for (int g = w; ok; g += 2) {
       // tiles that end before block g: hand (maximum, partial sum) to the epilogue and move on
       while (more && g >= g0 + nblk) {
-        if (n > 1) {   // the epilogue has read the values of the tile before the previous one
-          ok = __all_sync(0xffffffffu, wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1));
-          if (!ok) break;
+        if (n > 1) ok = __all_sync(0xffffffffu, wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1));   // tile n - 2's have been read
+        if (n >= 0 && ok) {
+          sh->lm[n & 1][w][r] = make_float2(m_mine, l);
+          mbar_arrive(b_lm_ready + 8 * (n & 1));
         }
-        sh->lm[n & 1][w][r] = make_float2(m_mine, l);
-        mbar_arrive(b_lm_ready + 8 * (n & 1));
         m_mine = -INFINITY;
         l = 0.f;
         g0 += nblk;
-        ++n;
-        map = next_regions(map, g0);
-        read_segment();
+        if (++n > 0) map = next_regions(map, g0);
+        const volatile Segment *seg = segment_at(n);
+        ok = __all_sync(0xffffffffu, ok && seg != nullptr);
         if (!ok) break;
+        more = seg->more;
+        nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
       }
       if (!ok || !more) break;
       const int j = g - g0;
@@ -838,16 +830,24 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 #pragma unroll
         for (int c = 0; c < kBN / 32; ++c) tmem_st16(tS + c * 16, zero);
       } else {
+        if (__any_sync(0xffffffffu, vis < kBN - 1)) {   // hidden columns, in place: once per tile or twice, so as little code as possible
+#pragma unroll 1
+          for (int c = 0; c < kBN; c += 16) {
+            uint32_t x[16];
+            tmem_ld16(tS + c, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = (c + k > vis) ? 0xff800000u : x[k];
+            tmem_st16(tS + c, x);
+          }
+          tmem_wait_st();
+        }
         uint32_t v[kBN];
         tmem_ld32p(tS, v);
         tmem_ld32p(tS + 32, v + 32);
         tmem_ld32p(tS + 64, v + 64);
         tmem_ld32p(tS + 96, v + 96);
         tmem_wait_ld();
-        if (vis < kBN - 1) {
-#pragma unroll
-          for (int c = 0; c < kBN; ++c) v[c] = (c > vis) ? 0xff800000u : v[c];
-        }
         // ---- row maximum: eight chains of three-input maxima ----
         float mc[8];
 #pragma unroll
