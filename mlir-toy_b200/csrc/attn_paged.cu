@@ -104,6 +104,11 @@ struct Args {
 constexpr size_t kPartO = static_cast<size_t>(kMaxCtas) * 2 * kBM * kD * sizeof(float);
 constexpr size_t kPartMl = static_cast<size_t>(kMaxCtas) * 2 * kBM * sizeof(float2);
 
+// New tokens of a sequence, where they sit and what there is to see.  Clamped, so that no device-side value leads out of
+// the tensors: rows stay inside [0, T), positions inside [-T - 1, len].
+struct Seq {
+  int first, n, pos, len;
+};
 struct Shared {
   uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
   uint64_t s_full[kSBufs], p_full[kSBufs], pv_done[kSBufs];
@@ -112,9 +117,10 @@ struct Shared {
   uint64_t sched_full[kSched];
   unsigned long long taint[2][kD];   // per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is not finite)
   unsigned scan[kThreads / 32];
-  unsigned before;                  // units in front of the sequence that the CTA's range begins in
+  unsigned before, units;                  // in front of the sequence that the CTA's range begins in, and its own
   Segment seg[kSched];
   int start_b;
+  Seq start_seq;                     // what that sequence brings
   int taint_any[2];                  // tile number + 1
   uint32_t tmem_base;
   int skip;
@@ -152,11 +158,6 @@ __device__ __forceinline__ bool wait_poll(uint32_t bar, uint32_t parity) {
   return false;
 }
 
-// New tokens of a sequence, where they sit and what there is to see.  Clamped, so that no device-side value leads out of
-// the tensors: rows stay inside [0, T), positions inside [-T - 1, len].
-struct Seq {
-  int first, n, pos, len;
-};
 __device__ __forceinline__ Seq seq_of(const Args &a, int b) {
   const int c0 = a.cu_seqlens[b], c1 = a.cu_seqlens[b + 1], len = a.seq_lens[b];
   Seq s;
@@ -225,7 +226,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   Shared *sh = reinterpret_cast<Shared *>(smem + kOffShared);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
   if (threadIdx.x < 2 * kD) sh->taint[threadIdx.x / kD][threadIdx.x % kD] = 0;
   if (warp == 15) {
     tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
@@ -236,11 +236,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
     sh->start_b = 0;
-    sh->before = 0;
+    sh->start_seq = Seq{0, 0, 0, 0};
+    sh->before = sh->units = 0;
     sh->taint_any[0] = sh->taint_any[1] = 0;
-    const int code = a.status ? *reinterpret_cast<volatile int *>(a.status) : 0;
-    sh->skip = (code != 0 && code != kErrTable && code != kErrSlot) ? 1 : 0;   // an expired wait, not refused data
-    a.owners[blockIdx.x].parts = 0;
   }
   if (warp == 13) {
     // one barrier per lane and turn
@@ -257,6 +255,15 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
     fence_barrier_init();
     fence_proxy_async_smem();
+  }
+
+  // Launched as a programmatic dependent: up to here the kernel before may still run.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
+  if (warp == 14 && lane == 0) {
+    const int code = a.status ? *reinterpret_cast<volatile int *>(a.status) : 0;
+    sh->skip = (code != 0 && code != kErrTable && code != kErrSlot) ? 1 : 0;   // an expired wait, not refused data
+    a.owners[blockIdx.x].parts = 0;
   }
 
   // ---- the CTA's range of the line: the units in front of each sequence ----
@@ -294,7 +301,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   auto claim = [&](int b) {                                    // the thread whose sequence holds unit r0
     if (idle || before > r0 || r0 >= before + mine) return;
     sh->start_b = b;
+    sh->start_seq = seq_of(a, b);
     sh->before = before;
+    sh->units = mine;
   };
   if (few) {
     if (lane == 31) claim(warp);
@@ -349,28 +358,22 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       int sb = 0, shd = 0, sj = 0, sblk = 0;
       unsigned at = r0;
       Seq seq{};
-      if (is_k) {
+      if (is_k && lane == 0) {
         sb = sh->start_b;
-        seq = seq_of(a, sb);
+        seq = sh->start_seq;
+        const unsigned per_head = sh->units / a.Hkv;
         unsigned rem = r0 - sh->before;
-        const unsigned sum = __shfl_sync(0xffffffffu, warp_scan(seq_units(seq, a.tok_tile, lane, 32), lane), 31);
-        shd = static_cast<int>(rem / max(sum, 1u));
-        rem -= shd * sum;
-        if (static_cast<unsigned>(shd) >= static_cast<unsigned>(a.Hkv)) at = r1;   // cu_seqlens is not a running sum: nothing to do
-        for (;; sj += 32 * a.tok_tile) {                   // 32 tiles at a time
-          const int j0 = sj + lane * a.tok_tile;
-          const unsigned units = j0 < seq.n ? tile_blocks(seq, j0, a.tok_tile) + kTileUnits : 0;
-          const unsigned incl = warp_scan(units, lane);
-          const unsigned past = __ballot_sync(0xffffffffu, incl > rem);
-          if (past) {
-            const int hit = __ffs(past) - 1;
-            sj += hit * a.tok_tile;
-            sblk = static_cast<int>(rem - __shfl_sync(0xffffffffu, incl - units, hit));
-            break;
-          }
-          rem -= __shfl_sync(0xffffffffu, incl, 31);
-          if (sj >= seq.n) break;                          // cannot be: rem is below the head's units
+        shd = static_cast<int>(rem / max(per_head, 1u));
+        if (shd >= a.Hkv) at = r1;                         // only if cu_seqlens is not a running sum: nothing to do
+        rem -= shd * per_head;
+#pragma unroll 1
+        while (sj < seq.n) {
+          const unsigned units = tile_blocks(seq, sj, a.tok_tile) + kTileUnits;
+          if (rem < units) break;
+          rem -= units;
+          sj += a.tok_tile;
         }
+        sblk = static_cast<int>(rem);
       }
       auto list_next = [&](int n) {                        // lane 0 of the K producer: tile n goes into the ring
         Segment w{};
@@ -932,34 +935,54 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 constexpr int kJoinWarps = 8;
 template <int DT> __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_join_kernel(const Args a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Owner own = a.owners[blockIdx.x];
   const int lane = threadIdx.x & 31;
   const int r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-  if (own.parts == 0 || r >= own.ntok * a.group) return;
   auto place = [&](int i) { return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kBM + r; };
+  const Owner own = a.owners[blockIdx.x];
+  const float2 first = a.part_ml[place(min(lane, kMaxCtas - 1 - static_cast<int>(blockIdx.x)))];   // asked for with the owner, used if there is a part
+  if (own.parts == 0 || r >= own.ntok * a.group) return;
+  // lane i holds (m, l) of parts i, i + 32, ...; m is a maximum that the part's weights are relative to
   float big = -INFINITY;
+#pragma unroll 1
   for (int i = lane; i < own.parts; i += 32) {
-    const float2 ml = a.part_ml[place(i)];
+    const float2 ml = i == lane ? first : a.part_ml[place(i)];
     if (ml.y != 0.f) big = fmaxf(big, ml.x);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < own.parts; ++i) {
-    const long long pr = place(i);
-    const float2 ml = a.part_ml[pr];
-    const float4 o = reinterpret_cast<const float4 *>(a.part_o + pr * kD)[lane];
-    if (ml.y != 0.f) {   // else the row saw nothing of this part
-      const float w = ex2(ml.x - big);
-      l = fmaf(w, ml.y, l);
-      acc.x = fmaf(w, o.x, acc.x);
-      acc.y = fmaf(w, o.y, acc.y);
-      acc.z = fmaf(w, o.z, acc.z);
-      acc.w = fmaf(w, o.w, acc.w);
+#pragma unroll 1
+  for (int i0 = 0; i0 < own.parts; i0 += 32) {
+    const int here = min(32, own.parts - i0);
+    float w = -1.f;                                       // of part i0 + lane; negative: the row saw nothing of it
+    if (lane < here) {
+      const float2 ml = i0 == 0 ? first : a.part_ml[place(i0 + lane)];
+      if (ml.y != 0.f) {
+        w = ex2(ml.x - big);
+        l = fmaf(w, ml.y, l);
+      }
+    }
+#pragma unroll 1
+    for (int i = 0; i < here; i += 8) {
+      float4 o[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i + k < here) o[k] = reinterpret_cast<const float4 *>(a.part_o + place(i0 + i + k) * kD)[lane];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, (i + k) & 31);
+        if (i + k < here && !(wk < 0.f)) {
+          acc.x = fmaf(wk, o[k].x, acc.x);
+          acc.y = fmaf(wk, o[k].y, acc.y);
+          acc.z = fmaf(wk, o[k].z, acc.z);
+          acc.w = fmaf(wk, o[k].w, acc.w);
+        }
+      }
     }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint4 *dst = a.out + static_cast<size_t>(own.tok0 + r / a.group) * a.out_t + static_cast<size_t>(own.kvh * a.group + r % a.group) * a.out_h;
   reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
@@ -993,18 +1016,21 @@ template <int DT> int launch(const CUtensorMap &tq, const CUtensorMap &tk, const
   int sms = 0, rc;
   if ((rc = device_sms<DT>(&sms)) != NB200_OK) return rc;
   const int grid = sms < kMaxCtas ? sms : kMaxCtas;
-  attn_paged_kernel<DT><<<dim3(grid), dim3(kThreads), kSmemBytes, st>>>(tq, tk, tv, a);
-  NB200_CHECK_CUDA(cudaGetLastError());
-  const int rows = a.T < a.tok_tile ? a.T * a.group : a.tok_tile * a.group;   // of the fullest tile
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps);
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = st;
   cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // both wait on the device for what is before them
   attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = st;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  NB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_paged_kernel<DT>, tq, tk, tv, a));
+  const int rows = a.T < a.tok_tile ? a.T * a.group : a.tok_tile * a.group;   // of the fullest tile
+  cfg.gridDim = dim3(grid, (rows + kJoinWarps - 1) / kJoinWarps);
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   NB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, attn_paged_join_kernel<DT>, a));
   return NB200_OK;
 }

@@ -111,6 +111,7 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
   constexpr int kSize = DT == NB200_F32 ? 4 : 2;
   __shared__ float4 turns[kWarps][kMaxHalf / 2];          // (cos, sin) of the token's angles, two to a word
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.wait;" ::: "memory");        // launched as a programmatic dependent
   const unsigned unit = blockIdx.x * kWarps + warp;
   if (unit >= units) return;
   const int t = static_cast<int>(unit / chunks), chunk = static_cast<int>(unit % chunks);
@@ -276,11 +277,18 @@ template <int DT, int G, bool APPEND> int launch_g(const Args &a, long long toke
   const long long chunks = (passes + per - 1) / per, units = tokens * chunks;
   NB200_REQUIRE(units < (1ll << 31), NB200_ERR_UNSUPPORTED, "norm and rotation: too many rows");
   const unsigned blocks = static_cast<unsigned>((units + kWarps - 1) / kWarps);
-  if (a.interleaved)
-    norm_rope_kernel<DT, G, APPEND, true><<<blocks, kThreads, 0, st>>>(a, static_cast<unsigned>(units), static_cast<unsigned>(chunks), static_cast<int>(per) * kRows);
-  else
-    norm_rope_kernel<DT, G, APPEND, false><<<blocks, kThreads, 0, st>>>(a, static_cast<unsigned>(units), static_cast<unsigned>(chunks), static_cast<int>(per) * kRows);
-  NB200_CHECK_CUDA(cudaGetLastError());
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the launch overlaps the end of the kernel before
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const unsigned n = static_cast<unsigned>(units), c = static_cast<unsigned>(chunks);
+  NB200_CHECK_CUDA(cudaLaunchKernelEx(&cfg, a.interleaved ? norm_rope_kernel<DT, G, APPEND, true> : norm_rope_kernel<DT, G, APPEND, false>,
+                                      a, n, c, static_cast<int>(per) * kRows));
   return NB200_OK;
 }
 template <int DT> int launch_dense(const Args &a, long long tokens, cudaStream_t st) {
