@@ -106,7 +106,7 @@ __device__ __forceinline__ int sequence_of(const int *cu, int B, int t, int lane
 // What bounds it beside HBM is the issue rate, so the arithmetic is on packed pairs of fp32, the weights are converted
 // once per token, and pointers advance by adding: 184 warp instructions per 32 / G rows went down to about 70.
 template <int DT, int G, bool APPEND, bool NEIGHBOURS>
-__global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, const unsigned units, const unsigned chunks, const int per) {
+__global__ void __launch_bounds__(kThreads, DT == NB200_F32 ? 5 : 7) norm_rope_kernel(const Args a, const unsigned units, const unsigned chunks, const int per) {
   constexpr int kRows = 32 / G;
   constexpr int kSize = DT == NB200_F32 ? 4 : 2;
   __shared__ float4 turns[kWarps][kMaxHalf / 2];          // (cos, sin) of the token's angles, two to a word
@@ -121,6 +121,34 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
   // byte offsets of the lane's two pieces
   const int e0 = (turned && !NEIGHBOURS ? 4 * u : 8 * u) * kSize, e1 = (turned && !NEIGHBOURS ? a.rot / 2 + 4 * u : 8 * u + 4) * kSize;
   const long long bt = APPEND ? 0 : t / a.S, st = APPEND ? t : t % a.S;
+
+  // The first rows' loads are in flight while the token's place and angles are looked up.
+  const int row_lo = chunk * per, row_hi = row_lo + per;
+  int kind = row_lo < a.Hq ? 0 : 1, lo = 0, hi = 0;        // queries, keys; the warp's rows of that kind
+  const char *src = nullptr;
+  long long src_step = 0;
+  piece_t<DT> x0[kUnroll], x1[kUnroll];
+  auto open = [&]() {
+    const int begin = kind ? a.Hq : 0;
+    lo = max(row_lo, begin);
+    hi = min(row_hi, kind ? a.Hq + a.Hkv : a.Hq);
+    const Strides &in = kind ? a.sk : a.sq;
+    src = static_cast<const char *>(kind ? a.k : a.q) + (bt * in.b + st * in.t + (lo - begin + sub) * in.h) * kSize + e0;
+    src_step = in.h * kRows * kSize;
+  };
+  auto fetch = [&](int row0) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) {
+      x0[i] = x1[i] = piece_t<DT>{};
+      if (in_row && row0 + i * kRows + sub < hi) {
+        x0[i] = load_piece<DT>(src, 0);
+        x1[i] = load_piece<DT>(src + (e1 - e0), 0);
+      }
+      src += src_step;
+    }
+  };
+  open();
+  fetch(lo);
 
   int pos = 0;
   long long slot_base = 0;                                // element offset of (page, head 0, row) in the pools
@@ -145,7 +173,6 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
     pos = a.positions[bt * a.positions_b + st];
   }
 
-  const int row_lo = chunk * per, row_hi = row_lo + per;
   if (row_lo < a.Hq + a.Hkv) {                            // else values alone
     for (int i = lane; i < a.rot / 2; i += 32) {
       const double x = static_cast<double>(pos) * static_cast<double>(a.inv_freq[i]) * 0.15915494309189535;   // 1 / 2 pi
@@ -166,13 +193,8 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
 
   // queries, then keys
 #pragma unroll 1
-  for (int kind = 0; kind < 2; ++kind) {
-    const int begin = kind ? a.Hq : 0, end = kind ? a.Hq + a.Hkv : a.Hq;
-    const int lo = max(row_lo, begin), hi = min(row_hi, end);
-    if (lo >= hi) continue;
-    const Strides in = kind ? a.sk : a.sq;
-    const char *src = static_cast<const char *>(kind ? a.k : a.q) + (bt * in.b + st * in.t + (lo - begin + sub) * in.h) * kSize + e0;
-    const long long src_step = in.h * kRows * kSize;
+  while (true) {
+    const int begin = kind ? a.Hq : 0;
     char *dst;
     long long dst_step;
     if (APPEND && kind) {
@@ -200,16 +222,7 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
       unpack(load_piece<DT>(static_cast<const char *>(w) + e0, 0), load_piece<DT>(static_cast<const char *>(w) + e1, 0), g);
 #pragma unroll 1
     for (int row0 = lo; row0 < hi; row0 += kUnroll * kRows) {
-      piece_t<DT> x0[kUnroll], x1[kUnroll];
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        x0[i] = x1[i] = piece_t<DT>{};
-        if (in_row && row0 + i * kRows + sub < hi) {
-          x0[i] = load_piece<DT>(src, 0);
-          x1[i] = load_piece<DT>(src + (e1 - e0), 0);
-        }
-        src += src_step;
-      }
+      if (row0 > lo) fetch(row0);
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
         if (row0 + i * kRows >= hi) break;                // the same for the whole warp
@@ -252,6 +265,10 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
         dst += dst_step;
       }
     }
+    if (kind == 1) break;
+    kind = 1;
+    open();
+    fetch(lo);
   }
   if constexpr (APPEND) {                                 // values: copied as they are
     const int begin = a.Hq + a.Hkv, lo = max(row_lo, begin), hi = min(row_hi, begin + a.Hkv);
@@ -269,9 +286,9 @@ __global__ void __launch_bounds__(kThreads, 7) norm_rope_kernel(const Args a, co
 // A warp does all the rows of a token where the tokens alone fill the SMs' warps; with fewer tokens their rows are dealt
 // out, down to one pass per warp, which then computes the token's angles again.
 template <int DT, int G, bool APPEND> int launch_g(const Args &a, long long tokens, int rows, cudaStream_t st) {
-  constexpr int kResident = 148 * 32, kRows = 32 / G;
+  constexpr int kResident = 148 * (DT == NB200_F32 ? 5 : 7) * kWarps, kRows = 32 / G;   // blocks to an SM by the launch bounds
   const int passes = (rows + kRows - 1) / kRows;
-  long long per = tokens * passes / kResident;
+  long long per = (tokens * passes + kResident - 1) / kResident;
   per = per < 1 ? 1 : (per >= passes ? passes : per);
   if (per > kUnroll) per = (per + kUnroll - 1) / kUnroll * kUnroll;
   const long long chunks = (passes + per - 1) / per, units = tokens * chunks;
