@@ -189,6 +189,11 @@ __device__ __forceinline__ unsigned warp_scan(unsigned x, int lane) {
   return x;
 }
 
+// A tile of at most 64 rows takes products of M = 64, whose rows lie 16 to a warp's 32 lanes.  Row of the tile at a lane of
+// the accumulator (128: none).
+__device__ __forceinline__ bool is_small(int ntok, int group) { return ntok * group <= 64; }
+__device__ __forceinline__ int row_at(int lane, bool small) { return !small ? lane : ((lane & 16) ? kBM : (lane >> 5) * 16 + (lane & 15)); }
+
 // Which TMEM region the three score buffers (bytes 0 to 2) and O (byte 3) are in.  Tile n > 0, whose first block is g,
 // takes the region of buffer (g + 2) % 3 for its O and leaves its predecessor's to that buffer.
 constexpr uint32_t kRegions = 0x03020100u;
@@ -501,7 +506,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // in a tile's third block also for the epilogue of the tile before, whose O that buffer takes over.
       if (lane == 0) {
         constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
-        constexpr uint32_t idesc_qk = umma_idesc_f16(fmt, 0, kBM, kBN);
         const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
         const uint32_t dq = static_cast<uint32_t>(umma_desc_sw128(sQ, 16, 1024)), dk = static_cast<uint32_t>(umma_desc_sw128(sK, 16, 1024));
         constexpr uint32_t kStageStep = kTileBytes >> 4;   // of buffer / stage 1
@@ -521,6 +525,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           ok = wait(b_q_full + 8 * (n & 1), (n >> 1) & 1);
           if (!ok) break;
           const uint32_t q_step = (n & 1) * kStageStep;
+          const uint32_t idesc_qk = is_small(seg->ntok, a.group) ? umma_idesc_f16(fmt, 0, kBM / 2, kBN) : umma_idesc_f16(fmt, 0, kBM, kBN);
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = wait(b_k_full + 8 * (g & 1), (g >> 1) & 1);
@@ -554,7 +559,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       // ================================ PV-product issuer ==================================
       if (lane == 0) {
         constexpr int fmt = (DT == NB200_BF16) ? 1 : 0;
-        constexpr uint32_t idesc_pv = umma_idesc_f16(fmt, 1, kBM, kD);
         // V is MN-major: 16 kv rows = 2 KB, the two 64-column halves kBox apart
         const uint32_t d_hi = static_cast<uint32_t>(umma_desc_sw128(0, 16, 1024) >> 32);
         const uint32_t dv = static_cast<uint32_t>(umma_desc_sw128(sV, kBox, 1024));
@@ -570,6 +574,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           const int nblk = seg->nblk, check = seg->check;
           if (n > 0) map = next_regions(map, g);
           const uint32_t o_tmem = tmem + region(map, 3);
+          const uint32_t idesc_pv = is_small(seg->ntok, a.group) ? umma_idesc_f16(fmt, 1, kBM / 2, kD) : umma_idesc_f16(fmt, 1, kBM, kD);
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = wait(b_v_full + 8 * (g & 1), (g >> 1) & 1);
@@ -607,15 +612,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int tok = r / a.group;
     // rows leave through a stage of 32 x 64 bytes per warp, four lanes to a row: whole sectors, eight rows to a store
     unsigned char *const stage = smem + kOffStage + (warp & 3) * kStage;
-    int out_row[4];                                          // token << 8 | head
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = (warp & 3) * 32 + 8 * i + (lane >> 2);
-      out_row[i] = (row / a.group) << 8 | (row % a.group);
-    }
     uint32_t looks = 0, notes = 0, map = kRegions;
     bool ok = true;
     // A tile's first two blocks are looked through before the epilogue of the tile before, which their products do not
@@ -684,6 +682,14 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       g0 += nblk;
       const int slot = seg->slot;
       const int ntok = seg->ntok;
+      const bool small = is_small(ntok, a.group);
+      const int tok = row_at(r, small) / a.group;
+      int out_row[4];                                        // token << 8 | head
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row_at((warp & 3) * 32 + 8 * i + (lane >> 2), small);
+        out_row[i] = (row / a.group) << 8 | (row % a.group);
+      }
       const int last_seen = min(seg->pos0 + tok, seg->len - 1);
       uint4 *const dst = a.out + static_cast<size_t>(seg->tok0) * a.out_t + static_cast<size_t>(seg->kvh * a.group) * a.out_h;
       const uint32_t tO = tmem + region(map, 3) + lane_addr;
@@ -709,9 +715,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const uint64_t inv2 = f2_pack(inv, inv);
       float *po = nullptr;
       if (slot >= 0) {
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + (warp & 3) * 32;
-        po = a.part_o + (pr + lane) * kD;
-        if (tok < ntok) a.part_ml[pr + lane] = make_float2(mf, l);
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + row_at(r, small);
+        po = a.part_o + pr * kD;
+        if (tok < ntok) a.part_ml[pr] = make_float2(mf, l);
       }
       ok = __all_sync(0xffffffffu, wait(b_o_full + 8 * (n & 3), (n >> 2) & 1));
       if (!ok) break;
@@ -758,7 +764,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       if (tainted) {   // columns whose values are not finite: NaN in the rows that see them
         __syncwarp();
-        uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(r % a.group) * a.out_h);
+        uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(row_at(r, small) % a.group) * a.out_h);
 #pragma unroll 1
         for (int c = 0; c < kD && tok < ntok; ++c) {
           const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
@@ -782,7 +788,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     const int w = warp >> 2;
     const int r = (warp & 3) * 32 + lane;                     // row in the tile == TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const int tok = r / a.group;
+    int tok = 0;
     int n = -1, g0 = 0;
     uint32_t map = kRegions;
     bool ok = true, more = true;
@@ -805,6 +811,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!ok) break;
         more = seg->more;
         nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
+        tok = row_at(r, is_small(ntok, a.group)) / a.group;
       }
       if (!ok || !more) break;
       const int j = g - g0;
