@@ -442,7 +442,10 @@ def test_chunk_attention_with_offsets_beyond_31_bits(cuda, native_lib):
     (torch.bfloat16, 40, 8, [(5 * i) % 8 for i in range(32)], [1 + (1237 * i) % 16001 for i in range(32)]),
     (torch.float16, 32, 8, [499] + [1] * 15, [4299] + [1 + (1811 * i) % 7600 for i in range(15)]),
     (torch.bfloat16, 16, 1, [300, 200, 5, 1], [6000, 200, 20000, 333]),
-], ids=["drafts", "mixed", "wide"])
+    (torch.bfloat16, 32, 8, [700], [17001]),                      # a cache beyond half the L2: tiles dealt out in waves
+    (torch.float16, 16, 16, [1300], [9003]),
+    (torch.bfloat16, 24, 8, [1536], [16512]),                     # tiles of 126 rows, no remainder behind the waves but one
+], ids=["drafts", "mixed", "wide", "document", "heads", "thirds"])
 def test_chunk_attention_streams_many_long_sequences(cuda, native_lib, dtype, Hq, Hkv, new, lens):
     """A cache larger than the L2: blocks arrive late and in bursts, while every CTA goes through parts of many tiles.
     The definition in 64 bits is evaluated on the device."""
