@@ -100,6 +100,7 @@ struct Args {
   uint4 *out;
   unsigned out_t, out_h;     // in 16 bytes
   int T, B, Hkv, group, tok_tile, num_pages, max_pages;
+  int inv_group;             // ceil(2^16 / group): row * inv_group >> 16 is row / group for rows of a tile
   float scale_log2;
   float *part_o;             // [kMaxCtas][2][128][128]
   float2 *part_ml;           // [kMaxCtas][2][128]
@@ -199,6 +200,7 @@ __device__ __forceinline__ unsigned warp_scan(unsigned x, int lane) {
 // A tile of at most 64 rows takes products of M = 64, whose rows lie 16 to a warp's 32 lanes.  Row of the tile at a lane of
 // the accumulator (128: none).
 __device__ __forceinline__ bool is_small(int ntok, int group) { return ntok * group <= 64; }
+__device__ __forceinline__ int token_of(const Args &a, int row) { return (row * a.inv_group) >> 16; }
 __device__ __forceinline__ int row_at(int lane, bool small) { return !small ? lane : ((lane & 16) ? kBM : (lane >> 5) * 16 + (lane & 15)); }
 
 // Which TMEM region the three score buffers (bytes 0 to 2) and O (byte 3) are in.  Tile n > 0, whose first block is g,
@@ -374,7 +376,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   };
 
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     if (warp == 12 || warp == 15) {
       // ================================ TMA producers ================================
       // warp 12: the list of tiles, Q of every tile and the K blocks; warp 15: the V blocks.  Lane i reads the table
@@ -386,64 +388,60 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int outside = a.num_pages * a.Hkv;             // a slice that the tensor map does not have: zeros
       // the scheduler's place: sequence, kv head, first token of the tile, block in it
       int sb = 0, shd = 0, sj = 0, sblk = 0;
-      unsigned at = r0;
+      unsigned at = 0;
       Seq seq{};
-      if (is_k && lane == 0) {
-        sb = sh->start_b;
-        seq = sh->start_seq;
-        const unsigned per_head = sh->units / a.Hkv;
-        unsigned rem = r0 - sh->before;
-        shd = static_cast<int>(rem / max(per_head, 1u));
-        if (shd >= a.Hkv) at = r1;                         // only if cu_seqlens is not a running sum: nothing to do
-        rem -= shd * per_head;
-#pragma unroll 1
-        while (sj < seq.n) {
-          const unsigned units = tile_blocks(seq, sj, a.tok_tile) + kTileUnits;
-          if (rem < units) break;
-          rem -= units;
-          sj += a.tok_tile;
-        }
-        sblk = static_cast<int>(rem);
-      }
-      auto fill = [&](Segment &w, int b, int h, const Seq &of, int j0, int blk0, int blocks) {
-        w.more = 1;
-        w.b = b, w.kvh = h;
-        w.tok0 = of.first + j0, w.ntok = min(a.tok_tile, of.n - j0);
-        w.pos0 = of.pos + j0, w.len = of.len;
-        w.blk0 = blk0, w.nblk = blocks;
-        w.check = max(max(min(w.pos0 + 1, w.len), 0) / kBN - blk0, 0);
-      };
       const int waves = sh->waves;
       auto list_next = [&](int n) {                        // lane 0 of the K producer: tile n goes into the ring
         Segment w{};
-        if (n < waves) {                                   // of the only sequence
-          const Seq only = sh->start_seq;
-          const unsigned t = n * gridDim.x + blockIdx.x, tiles = (only.n + a.tok_tile - 1) / a.tok_tile;
-          const int h = static_cast<int>(t / tiles), j0 = static_cast<int>(t - h * tiles) * a.tok_tile;
-          fill(w, 0, h, only, j0, 0, tile_blocks(only, j0, a.tok_tile));
-          w.slot = -1;
-          sh->seg[n % kSched] = w;
-          mbar_arrive(b_sched + 8 * (n % kSched));
-          return;
+        unsigned stop = r1;
+        if (n <= waves) {
+          // tile n of the waves, which are of the only sequence, or the place where the CTA's range of the line begins
+          sb = sh->start_b;
+          seq = sh->start_seq;
+          const unsigned in_head = n < waves ? (seq.n + a.tok_tile - 1) / a.tok_tile : sh->units / a.Hkv;
+          unsigned rem = n < waves ? n * gridDim.x + blockIdx.x : r0 - sh->before;
+          shd = static_cast<int>(rem / max(in_head, 1u));
+          rem -= shd * in_head;
+          sj = sblk = 0;
+          if (n < waves) {
+            sj = static_cast<int>(rem) * a.tok_tile;
+            at = 0;
+            stop = 0x7fffffffu;
+          } else {
+            at = r0;
+            if (shd >= a.Hkv) at = r1;                     // the waves were all, or cu_seqlens is not a running sum
+#pragma unroll 1
+            while (sj < seq.n) {
+              const unsigned units = tile_blocks(seq, sj, a.tok_tile) + kTileUnits;
+              if (rem < units) break;
+              rem -= units;
+              sj += a.tok_tile;
+            }
+            sblk = static_cast<int>(rem);
+          }
         }
-        while (at < r1) {
+#pragma unroll 1
+        while (at < stop) {
           if (sj >= seq.n) {                               // on to the next kv head, or sequence with new tokens
             sj = 0;
             if (++shd == a.Hkv) {
               shd = 0;
+#pragma unroll 1
               do {
                 if (++sb < a.B) seq = seq_of(a, sb);
               } while (seq.n == 0 && sb < a.B);
-              if (sb >= a.B) {                             // not with a running sum in cu_seqlens
-                at = r1;
-                break;
-              }
+              if (sb >= a.B) break;                        // not with a running sum in cu_seqlens
             }
           }
           const int blocks = tile_blocks(seq, sj, a.tok_tile);
           if (sblk < blocks) {
-            const int take = static_cast<int>(min(static_cast<unsigned>(blocks - sblk), r1 - at));
-            fill(w, sb, shd, seq, sj, sblk, take);
+            const int take = static_cast<int>(min(static_cast<unsigned>(blocks - sblk), stop - at));
+            w.more = 1;
+            w.b = sb, w.kvh = shd;
+            w.tok0 = seq.first + sj, w.ntok = min(a.tok_tile, seq.n - sj);
+            w.pos0 = seq.pos + sj, w.len = seq.len;
+            w.blk0 = sblk, w.nblk = take;
+            w.check = max(max(min(w.pos0 + 1, w.len), 0) / kBN - sblk, 0);
             w.slot = take == blocks ? -1 : (sblk > 0 ? 0 : 1);
             if (w.slot == 1) {                             // goes on in the CTAs up to the one that has its last block
               const unsigned x = at + blocks - 1 - base_units, longer = more_until * (share + 1);
@@ -648,7 +646,6 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     }
   } else if (warp >= 8) {
     // ================================ epilogue: O / l -> out, or (O, m, l) -> workspace ==========================
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
     // rows leave through a stage of 32 x 64 bytes per warp, four lanes to a row: whole sectors, eight rows to a store
@@ -722,12 +719,12 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const int slot = seg->slot;
       const int ntok = seg->ntok;
       const bool small = is_small(ntok, a.group);
-      const int tok = row_at(r, small) / a.group;
+      const int row = row_at(r, small), tok = token_of(a, row);
       int out_row[4];                                        // token << 8 | head
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = row_at((warp & 3) * 32 + 8 * i + (lane >> 2), small);
-        out_row[i] = (row / a.group) << 8 | (row % a.group);
+        const int row = row_at((warp & 3) * 32 + 8 * i + (lane >> 2), small), tok = token_of(a, row);
+        out_row[i] = tok << 8 | (row - tok * a.group);
       }
       const int last_seen = min(seg->pos0 + tok, seg->len - 1);
       uint4 *const dst = a.out + static_cast<size_t>(seg->tok0) * a.out_t + static_cast<size_t>(seg->kvh * a.group) * a.out_h;
@@ -754,7 +751,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       const uint64_t inv2 = f2_pack(inv, inv);
       float *po = nullptr;
       if (slot >= 0) {
-        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + row_at(r, small);
+        const long long pr = (static_cast<long long>(blockIdx.x) * 2 + slot) * kBM + row;
         po = a.part_o + pr * kD;
         if (tok < ntok) a.part_ml[pr] = make_float2(mf, l);
       }
@@ -803,7 +800,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       }
       if (tainted) {   // columns whose values are not finite: NaN in the rows that see them
         __syncwarp();
-        uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(row_at(r, small) % a.group) * a.out_h);
+        uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(row - tok * a.group) * a.out_h);
 #pragma unroll 1
         for (int c = 0; c < kD && tok < ntok; ++c) {
           const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
@@ -823,7 +820,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     if (!ok && lane == 0) report(a.status, kErrEpilogue, g0);
   } else {
     // ================================ softmax: warpgroup w takes the blocks g with g & 1 == w ================
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
     const int w = warp >> 2;
     const int r = (warp & 3) * 32 + lane;                     // row in the tile == TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -833,8 +830,10 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     bool ok = true, more = true;
     int nblk = 0, blk0 = 0, pos0 = 0, len = 0, ntok = 0;
     float m_mine = -INFINITY, l = 0.f;
+#pragma unroll 1
     for (int g = w; ok; g += 2) {
       // tiles that end before block g: hand (maximum, partial sum) to the epilogue and move on
+#pragma unroll 1
       while (more && g >= g0 + nblk) {
         if (n > 1) ok = __all_sync(0xffffffffu, wait(b_lm_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1));   // tile n - 2's have been read
         if (n >= 0 && ok) {
@@ -850,7 +849,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!ok) break;
         more = seg->more;
         nblk = seg->nblk, blk0 = seg->blk0, pos0 = seg->pos0, len = seg->len, ntok = seg->ntok;
-        tok = row_at(r, is_small(ntok, a.group)) / a.group;
+        tok = token_of(a, row_at(r, is_small(ntok, a.group)));
       }
       if (!ok || !more) break;
       const int j = g - g0;
@@ -891,25 +890,24 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           tmem_wait_st();
         }
-        uint32_t v[kBN];
-        tmem_ld32p(tS, v);
-        tmem_ld32p(tS + 32, v + 32);
-        tmem_ld32p(tS + 64, v + 64);
-        tmem_ld32p(tS + 96, v + 96);
-        tmem_wait_ld();
-        // ---- row maximum: eight chains of three-input maxima ----
+        // Two passes over the scores, read from tensor memory 64 columns at a time: holding all 128 in registers takes 176 of
+        // them, which the epilogue and the producers then lack, and twice the code (176 against 164 us at a 4096-token
+        // first chunk under sustained load).
         float mc[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          mc[c] = max3(__uint_as_float(v[c * 16]), __uint_as_float(v[c * 16 + 1]), __uint_as_float(v[c * 16 + 2]));
+        for (int c = 0; c < 8; ++c) mc[c] = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[64];
+          tmem_ld32p(tS + h * 64, v);
+          tmem_ld32p(tS + h * 64 + 32, v + 32);
+          tmem_wait_ld();
 #pragma unroll
-        for (int k = 3; k + 1 < 16; k += 2) {
+          for (int k = 0; k < 8; k += 2) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            mc[c] = max3(mc[c], __uint_as_float(v[c * 16 + k]), __uint_as_float(v[c * 16 + k + 1]));
+            for (int c = 0; c < 8; ++c) mc[c] = max3(mc[c], __uint_as_float(v[c * 8 + k]), __uint_as_float(v[c * 8 + k + 1]));
+          }
         }
-#pragma unroll
-        for (int c = 0; c < 8; ++c) mc[c] = fmaxf(mc[c], __uint_as_float(v[c * 16 + 15]));
         const float mx = fmaxf(max3(mc[0], mc[1], mc[2]), fmaxf(max3(mc[3], mc[4], mc[5]), fmaxf(mc[6], mc[7])));
         const float m_blk = mx * a.scale_log2;                   // -inf if the row sees nothing of this block
         // ---- the maximum to use: the one block g-1 decided on, unless this block exceeds it by more than 2^8 ----
@@ -943,19 +941,26 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         const float m_use = m_new == -INFINITY ? 0.f : m_new;    // nothing seen so far: every p is 2^(-inf) = 0
         const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
         uint64_t lsum2 = f2_pack(0.f, 0.f);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[64];
+          tmem_ld32p(tS + h * 64, v);
+          tmem_ld32p(tS + h * 64 + 32, v + 32);
+          tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kBN / 32; ++c) {
-          uint32_t pk[16];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const uint64_t x2 = f2_fma(
-                f2_pack(__uint_as_float(v[c * 32 + 2 * k]), __uint_as_float(v[c * 32 + 2 * k + 1])), c2, nm2);
-            const float2 x = f2_unpack(x2);
-            const float p0 = ex2(x.x), p1 = ex2(x.y);
-            lsum2 = f2_add(lsum2, f2_pack(p0, p1));
-            pk[k] = pack2<DT>(p0, p1);
+            for (int k = 0; k < 16; ++k) {
+              const uint64_t x2 = f2_fma(
+                  f2_pack(__uint_as_float(v[c * 32 + 2 * k]), __uint_as_float(v[c * 32 + 2 * k + 1])), c2, nm2);
+              const float2 x = f2_unpack(x2);
+              const float p0 = ex2(x.x), p1 = ex2(x.y);
+              lsum2 = f2_add(lsum2, f2_pack(p0, p1));
+              pk[k] = pack2<DT>(p0, p1);
+            }
+            tmem_st16(tS + h * 32 + c * 16, pk);
           }
-          tmem_st16(tS + c * 16, pk);
         }
         const float2 ls = f2_unpack(lsum2);
         l += ls.x + ls.y;
@@ -1030,7 +1035,7 @@ template <int DT> __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint4 *dst = a.out + static_cast<size_t>(own.tok0 + r / a.group) * a.out_t + static_cast<size_t>(own.kvh * a.group + r % a.group) * a.out_h;
+  uint4 *dst = a.out + static_cast<size_t>(own.tok0 + token_of(a, r)) * a.out_t + static_cast<size_t>(own.kvh * a.group + r - token_of(a, r) * a.group) * a.out_h;
   reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
 }
 
@@ -1126,7 +1131,7 @@ extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *
   Args a{};
   a.block_table = block_table, a.cu_seqlens = cu_seqlens, a.seq_lens = seq_lens;
   a.out = static_cast<uint4 *>(out), a.out_t = static_cast<unsigned>(s[2] / 8), a.out_h = static_cast<unsigned>(s[3] / 8);
-  a.T = T, a.B = B, a.Hkv = Hkv, a.group = Hq / Hkv, a.tok_tile = kBM / a.group;
+  a.T = T, a.B = B, a.Hkv = Hkv, a.group = Hq / Hkv, a.tok_tile = kBM / a.group, a.inv_group = ((1 << 16) + a.group - 1) / a.group;
   a.num_pages = num_pages, a.max_pages = max_pages, a.scale_log2 = scale_log2, a.status = status;
   char *ws = static_cast<char *>(workspace);
   a.part_o = reinterpret_cast<float *>(ws);
