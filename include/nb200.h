@@ -75,7 +75,7 @@ int nb200_attn_fwd(const void *q, const void *k, const void *v, void *out,
  * code 23: an appended row whose position its block-table row does not reach),
  * NB200_ERR_DEVICE_TIMEOUT for every other code (an expired bounded wait). host_out may be NULL.
  * A non-zero status[0] makes later attention and SSD launches that are given the same buffer return at once
- * without touching their outputs, so read it (and zero it) after synchronising whenever a result matters. */
+ * without touching their outputs (nb200_attn_paged: codes 22 and 23, refused data, do not), so read it (and zero it) after synchronising whenever a result matters. */
 int nb200_status_read(const int *status, int *host_out, void *stream);
 
 /*
@@ -283,7 +283,8 @@ int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, c
  *   cu_seqlens : int32 [B + 1], not decreasing      seq_lens : int32 [B]
  *   q_weight, k_weight, inv_freq, rot_dim, interleaved, eps : as for nb200_qk_norm_rope
  *   strides    : HOST array of 8: the token and head stride (in elements) of q, k, v and q_out; rules as above
- * Rows that belong to no sequence (before cu_seqlens[0], from cu_seqlens[B] on) are not touched, in q_out as in the
+ * T is at least 1, T * (Hq + 2 Hkv) below 2^31; the call is one kernel, launched as a programmatic dependent of the one
+ * before it on the stream.  Rows that belong to no sequence (before cu_seqlens[0], from cu_seqlens[B] on) are not touched, in q_out as in the
  * cache.  Of a row whose position is outside its row of the block table, or whose page is outside the pool, nothing
  * is written and `status` (may be NULL) records code 23 with the row and the position, or code 22 with the entry, which
  * nb200_status_read reports as NB200_ERR_BAD_ARG.  Two sequences of one call must not append to the same page.
@@ -306,8 +307,12 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out: multiples of 16 bytes, at least a row (the
  *                stride of an extent of 1 is not used)
  *   scale_log2 : log2(e) * softmax scale
+ * At most 128 query heads to a kv head; T below 2^30, max_pages * page_size up to 2^30.  Two kernels: the second joins the
+ * tiles that were worked on by more than one CTA, in an order that lengths alone decide, so that equal calls give equal
+ * bits.  out shares no element with the other tensors.
  * A row that sees nothing (its position is negative) is 0; rows that belong to no sequence are not touched.  Cache rows
- * at and beyond a sequence's length are not used, whatever they hold.  A table entry outside [0, num_pages) is never
+ * at and beyond a sequence's length are not used, whatever they hold; a value that is infinite or NaN makes that column
+ * of the rows that see it not finite, and reaches no other row.  A table entry outside [0, num_pages) is never
  * dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and
  * `status` records code 22.
  */

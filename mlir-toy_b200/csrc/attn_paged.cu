@@ -158,14 +158,6 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
     if (mbar_try_wait_suspend(bar, parity, 1000u)) return true;
   return false;
 }
-// The same without suspending (test_wait): the waiter goes on a few cycles after the phase completes.  For an issuing thread.
-__device__ __forceinline__ bool wait_poll(uint32_t bar, uint32_t parity) {
-#pragma unroll 1
-  for (int i = 0; i < 1 << 26; ++i)
-    if (mbar_test_wait(bar, parity)) return true;
-  return false;
-}
-
 __device__ __forceinline__ Seq seq_of(const Args &a, int b) {
   const int c0 = a.cu_seqlens[b], c1 = a.cu_seqlens[b + 1], len = a.seq_lens[b];
   Seq s;
@@ -573,7 +565,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               ++freed;
             }
             if (g >= kSBufs) {
-              ok = wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1);
+              ok = wait(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1);
               if (!ok) break;
             }
             tc_fence_after();
@@ -625,7 +617,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
               if (!ok) break;
               looks ^= 1u << (g & 1);
             }
-            ok = wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1);
+            ok = wait(b_p_full + 8 * sb, (g / kSBufs) & 1);
             if (!ok) break;
             tc_fence_after();
             const uint32_t p_tmem = tmem + region(map, sb), v_at = dv + (g & 1) * kStageStep;

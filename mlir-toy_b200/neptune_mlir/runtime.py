@@ -208,6 +208,13 @@ def _refuse(what: str):
     raise ValueError(f"{what}: the tensors do not fit the arguments")   # the checks before this name the tensor
 
 
+def _first_status_buffer(dev: torch.device) -> None:
+    """Make a device's status words; not inside a graph capture, whose memory ends with the graph."""
+    if dev.index not in _status_buffers and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the first call on a device makes its status words: call once before capturing a graph")
+    status_buffer(dev)
+
+
 def _weight_checks(weights, D: int, dtype: str) -> list:
     """Check the norm weights that are there; return them."""
     there = [(name, w) for name, w in zip(("q_weight", "k_weight"), weights) if w is not None]
@@ -276,7 +283,7 @@ def rope_append(q, k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, in
         _check("inv_freq", inv_freq, (rot_dim // 2,), torch.float32)
         dev = _same_device(k, v, k_pages, v_pages, block_table, cu_seqlens, seq_lens, inv_freq,
                            *_weight_checks((q_weight, k_weight), D, dtype), *((q, q_out) if Hq else ()))
-        status_buffer(dev)                                       # the first call on a device makes its status words
+        _first_status_buffer(dev)
         rc = native.binding().rope_append(*args)
         if rc is None:
             _refuse("rope_append")
@@ -308,7 +315,7 @@ def attn_paged(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace
         if not (isinstance(workspace, torch.Tensor) and workspace.is_cuda and workspace.is_contiguous()
                 and workspace.numel() * workspace.element_size() >= need):
             raise ValueError(f"workspace: need a contiguous CUDA tensor of at least {need} bytes")
-        status_buffer(_same_device(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out))
+        _first_status_buffer(_same_device(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, workspace, out))
         rc = native.binding().attn_paged(*args)
         if rc is None:
             _refuse("attn_paged")

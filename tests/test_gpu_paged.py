@@ -351,6 +351,10 @@ def test_chunk_attention_with_strided_queries_and_output(cuda, native_lib):
     finish()
     check_attention(batch, x[:, 2 * D:10 * D].unflatten(-1, (8, D)), out)
     assert bool((wide[..., :D] == 7.0).all())
+    heads = x[:, 2 * D:10 * D].unflatten(-1, (8, D)).transpose(0, 1).contiguous().to(cuda)   # head-major queries
+    out = attend(batch, heads.transpose(0, 1), cuda)
+    finish()
+    check_attention(batch, x[:, 2 * D:10 * D].unflatten(-1, (8, D)), out)
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=NAMES.get)
