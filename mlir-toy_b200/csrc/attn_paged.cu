@@ -8,16 +8,18 @@
 // group heads (row = token * group + head).  Tiles run over sequence, kv head, chunk of tokens; each has a number of KV
 // blocks of 128 rows (two pages) that follows from the device-side lengths.  The blocks of all tiles form one line, which
 // is cut into equal ranges, one per CTA: a few drafted tokens over one long cache keep every SM as busy as a long prompt
-// does, and all CTAs end together, whatever the lengths.  (One exception: see kWaveBytes.)  A range that covers a whole tile writes its output; the (at
-// most two) tiles that a CTA has in part leave un-normalised fp32 partials (o, m, l), which a second kernel joins in
-// the order of the line, so results do not depend on timing.
+// does, and all CTAs end together, whatever the lengths.  (One exception: see kWaveBytes.)  A range that covers a whole
+// tile writes its output; the (at most two) tiles that a CTA has in part leave un-normalised fp32 partials (o, m, l),
+// which a second kernel joins in the order of the line, so results do not depend on timing.
 //
 // Inside a CTA the blocks of its ranges form one stream, numbered g = 0, 1, 2, ..., that does not stop at tile borders:
 //
 //   S(g) = Q K(g)^T      8 x tcgen05.mma 128x128x16, both operands in shared memory, into TMEM buffer g % 3
-//   softmax(g)           warpgroup g & 1 (thread = row = TMEM lane): scores to registers, row maximum, p = 2^(s - m),
-//                        P(g) as packed 16-bit over the first 64 columns of the same TMEM buffer
+//   softmax(g)           warpgroup g & 1 (thread = row = TMEM lane): row maximum, p = 2^(s - m), P(g) as packed 16-bit
+//                        over the first 64 columns of the same TMEM buffer
 //   O += P(g) V(g)       8 x tcgen05.mma 128x128x16 with P read from TMEM
+//
+// (64x128x16 for a tile of at most 64 rows: no faster, but the products' power counts where the clock is at the limit.)
 //
 //   warps 0-3 / 4-7  softmax of even / odd blocks      warps 8-11   epilogue
 //   warp 12, 15      TMA producers: Q and K (and the list of tiles); V (warp 15 also allocates the 512 TMEM columns)
@@ -26,9 +28,14 @@
 // The 512 TMEM columns are four regions of 128: three score buffers and O.  Reading a finished O takes the epilogue 2 to 3
 // us, and a tile of a chunk may be over in two blocks, so the next tile does not wait for it: its O takes over the region
 // of the score buffer whose turn comes last, and that buffer moves to the old O's region once it has been read, two blocks
-// later.  (Waiting cost 4.5 us a tile: 223 us for a 4096-token first chunk.)  What bounds a block then is the chain from
-// PV(g-3) over S(g) and its softmax to PV(g), 2.6 us for three blocks in flight; a third stage for K and V in place of
-// Q's second buffer changed nothing.
+// later.
+//
+// What bounds it.  A block takes 0.9 us where its products need 0.53: three blocks are in flight and the chain from PV(g-3)
+// over S(g) and its softmax to PV(g) is 2.6 us long.  A change of tiles costs about 2 us more.  Under sustained load the
+// power limit takes the clock from 1.9 to 1.3 - 1.5 GHz and both grow with it.  Measured, 32 / 8 heads, bf16:
+//   4096 tokens, nothing cached     141 us alone (975 TFLOP/s), 160 sustained; tensor pipe 48 % busy
+//   2048 tokens over 30000 rows     850 us alone (1250 TFLOP/s), 955 sustained
+//   32 sequences of up to 7 tokens, 40 / 8 heads, up to 16001 rows: 166 us, 1.04 GB read once at 6.3 TB/s; 176 sustained
 //
 // P is rounded to the storage type because the second product takes both operands in one 16-bit type; the row sum adds
 // the unrounded values.  The running maximum passes between the warpgroups through shared memory, O is rescaled only when
@@ -39,8 +46,7 @@
 // may hold anything there.  V may not, since 0 * NaN is NaN: in the blocks that some row of the tile does not see
 // whole, the epilogue warps (idle then) clear V rows behind the sequence's end in shared memory, and look for infinities
 // and NaN in the rows that only some of the tile's rows see, before the PV product of that block.  Such a value is
-// replaced by 0 and noted; the epilogue makes it a NaN in exactly those rows that see it.  Done by the softmax warps, the
-// same look cost 44 of 211 us at a 4096-token first chunk.
+// replaced by 0 and noted; the epilogue makes it a NaN in exactly those rows that see it.
 //
 // Every wait is bounded; on expiry the role records a code in the status words and unwinds.
 #include <cuda.h>
@@ -73,7 +79,8 @@ constexpr int kMaxCtas = 160;                   // CTAs that the workspace has r
 // Cut like that, the CTAs of a head are all over its K and V at any time, which is fine while those stay in the L2.  A
 // single sequence whose K and V do not, and whose tiles are about equally long, is dealt out in waves first: every CTA
 // takes the same number of whole tiles, in order, so that neighbours read the same blocks at the same time, and only what
-// is left is cut.  2048 tokens over 30000 cached rows (131 MB): 2.46 GB of DRAM reads without, 1113 us under sustained load.
+// is left is cut.  2048 tokens over 30000 cached rows (131 MB): 0.15 GB of DRAM reads and 971 us under sustained load, 2.46 GB
+// and 1117 us without.
 constexpr long long kWaveBytes = 1ll << 26;     // half of the L2
 constexpr int kTileUnits = 2;                   // what changing tiles costs (2 us), in blocks, on the line that is cut
 
@@ -884,7 +891,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         // Two passes over the scores, read from tensor memory 64 columns at a time: holding all 128 in registers takes 176 of
         // them, which the epilogue and the producers then lack, and twice the code (176 against 164 us at a 4096-token
-        // first chunk under sustained load).
+        // first chunk under sustained load, and 120 against 100 us for 512 sequences of 32 tokens over 128 rows).
         float mc[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) mc[c] = -INFINITY;
