@@ -652,7 +652,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     uint32_t looks = 0, notes = 0, map = kRegions;
     bool ok = true;
     // A tile's first two blocks are looked through before the epilogue of the tile before, which their products do not
-    // wait for; its further blocks after it, because their scores do.
+    // wait for; its further blocks after it, because their scores do.  (A tile's tokens are at no more than 128 positions,
+    // so the blocks to look through are its last two at most, and the next tile is listed before they are waited for:
+    // listing it takes the issue of the tile's last K block, which waits for the PV product of the sixth last.)
     int g0 = 0, done = 0;                                    // first block of tile n, its blocks looked through
     for (int n = 0; ok; ++n) {
       const volatile Segment *seg = segment_at(n);
