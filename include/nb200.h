@@ -75,7 +75,8 @@ int nb200_attn_fwd(const void *q, const void *k, const void *v, void *out,
  * code 23: an appended row whose position its block-table row does not reach),
  * NB200_ERR_DEVICE_TIMEOUT for every other code (an expired bounded wait). host_out may be NULL.
  * A non-zero status[0] makes later attention and SSD launches that are given the same buffer return at once
- * without touching their outputs (nb200_attn_paged: codes 22 and 23, refused data, do not), so read it (and zero it) after synchronising whenever a result matters. */
+ * without touching their outputs (codes 22 and 23, refused data, do not stop nb200_attn_paged), so read it (and zero it)
+ * after synchronising whenever a result matters. */
 int nb200_status_read(const int *status, int *host_out, void *stream);
 
 /*
@@ -264,7 +265,8 @@ int nb200_decode_fwd_static(const void *q, const void *k, const void *v, void *o
  *               then the batch stride of positions (0: one row for all).  Rows are contiguous; strides and base
  *               addresses are multiples of 16 bytes.  So q and k may be views into a packed projection and q_out,
  *               k_out [B, H, S, D] tensors as nb200_attn_fwd reads them.
- * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.
+ * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.  An output's
+ * rows lie apart: a stride smaller than a row is refused, unless its extent is 1.
  */
 int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, const int *positions,
                        const float *inv_freq, const void *q_weight, const void *k_weight, const long long *strides,
@@ -288,7 +290,7 @@ int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, c
  * cache.  Of a row whose position is outside its row of the block table, or whose page is outside the pool, nothing
  * is written and `status` (may be NULL) records code 23 with the row and the position, or code 22 with the entry, which
  * nb200_status_read reports as NB200_ERR_BAD_ARG.  Two sequences of one call must not append to the same page.
- * q_out may be q (same address and strides); otherwise outputs share no element with inputs.
+ * q_out may be q (same address and strides), its rows apart as above; otherwise outputs share no element with inputs.
  */
 int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, void *k_pages, void *v_pages,
                       const int *block_table, const int *cu_seqlens, const int *seq_lens, const float *inv_freq,

@@ -444,7 +444,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             w.slot = take == blocks ? -1 : (sblk > 0 ? 0 : 1);
             if (w.slot == 1) {                             // goes on in the CTAs up to the one that has its last block
               const unsigned x = at + blocks - 1 - base_units, longer = more_until * (share + 1);
-              const unsigned last = x < longer ? x / (share + 1) : more_until + (x - longer) / share;
+              // (the bound holds back only a cu_seqlens whose sequences overlap so often that the units wrapped around)
+              const unsigned last = min(x < longer ? x / (share + 1) : more_until + (x - longer) / share, gridDim.x - 1);
               a.owners[blockIdx.x] = Owner{static_cast<int>(last - blockIdx.x) + 1, w.kvh, w.tok0, w.ntok};
             }
             at += take;

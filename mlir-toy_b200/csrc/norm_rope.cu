@@ -325,6 +325,13 @@ int check_view(const char *who, const char *name, const void *p, const Strides &
                 "%s: the strides of %s must be multiples of 16 bytes", who, name);
   return NB200_OK;
 }
+// An output's rows must not lie over one another, as those of an expanded tensor do.
+int check_rows_apart(const char *who, const char *name, const Strides &s, int B, int S, int H, int D) {
+  auto apart = [&](int extent, long long stride) { return extent == 1 || stride >= D || stride <= -D; };
+  NB200_REQUIRE(apart(B, s.b) && apart(S, s.t) && apart(H, s.h), NB200_ERR_BAD_ARG,
+                "%s: the strides of %s must be at least a row", who, name);
+  return NB200_OK;
+}
 int check_rotation(const char *who, int D, int rot, float eps) {
   NB200_REQUIRE(rot >= 16 && rot <= D && rot % 16 == 0, NB200_ERR_UNSUPPORTED,
                 "%s: rot_dim = %d, a multiple of 16 from 16 to D = %d is needed", who, rot, D);
@@ -358,6 +365,7 @@ extern "C" int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, voi
   for (int i = 0; i < 4; ++i) {
     *views[i] = Strides{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
     if ((rc = check_view(who, names[i], ptrs[i], *views[i], size)) != NB200_OK) return rc;
+    if (i >= 2 && (rc = check_rows_apart(who, names[i], *views[i], B, S, i == 2 ? Hq : Hkv, D)) != NB200_OK) return rc;
   }
   NB200_REQUIRE((!q_weight || aligned16(q_weight)) && (!k_weight || aligned16(k_weight)), NB200_ERR_BAD_ARG,
                 "%s: the weights must be 16-byte aligned", who);
@@ -399,6 +407,7 @@ extern "C" int nb200_rope_append(const void *q, const void *k, const void *v, vo
     if (Hq == 0 && (i == 0 || i == 3)) continue;
     *views[i] = Strides{0, strides[2 * i], strides[2 * i + 1]};
     if ((rc = check_view(who, names[i], ptrs[i], *views[i], 2)) != NB200_OK) return rc;
+    if (i == 3 && (rc = check_rows_apart(who, names[i], *views[i], 1, T, Hq, D)) != NB200_OK) return rc;
   }
   NB200_REQUIRE(aligned16(k_pages) && aligned16(v_pages), NB200_ERR_BAD_ARG, "%s: the page pools must be 16-byte aligned", who);
   NB200_REQUIRE((!q_weight || aligned16(q_weight)) && (!k_weight || aligned16(k_weight)), NB200_ERR_BAD_ARG,

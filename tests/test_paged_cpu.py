@@ -76,6 +76,23 @@ def test_attn_paged_rejects_bad_calls_without_a_gpu(native_lib, ptr):
         assert call(**kwargs) == code and text in lib.nb200_last_error(), kwargs
 
 
+def test_outputs_whose_rows_lie_over_one_another_are_refused(native_lib, ptr):
+    lib, p = native.load(str(native_lib)), ptr[0]
+
+    def norm_rope(q_out, k_out=(2048, 256, 128), B=2, S=8):
+        strides = longs(2048, 256, 128, 2048, 256, 128, *q_out, *k_out, 0)
+        return lib.nb200_qk_norm_rope(p, p, p, p, p, p, None, None, strides, B, S, 2, 2, 128, 128, 0, 1e-6, 1, None)
+
+    def append(q_out):
+        return lib.nb200_rope_append(p, p, p, p, p, p, p, p, p, p, None, None, longs(256, 128, 256, 128, 256, 128, *q_out), 2, 1,
+                                     2, 2, 8, 4, 64, 128, 128, 0, 1e-6, 1, None, None)
+
+    for call, args, name in ((norm_rope, [(0, 256, 128)], b"q_out"), (norm_rope, [(2048, 0, 128)], b"q_out"),
+                             (norm_rope, [(2048, 256, 64)], b"q_out"), (norm_rope, [(2048, 256, 128), (2048, 256, 0)], b"k_out"),
+                             (append, [(0, 128)], b"q_out"), (append, [(256, 120)], b"q_out")):
+        assert call(*args) == -1 and b"strides of " + name + b" must be at least a row" in lib.nb200_last_error(), args
+
+
 def test_runtime_refuses_cpu_tensors(native_lib):
     x = torch.zeros((1, 4, 2, 128), dtype=torch.bfloat16)
     i = torch.zeros((4,), dtype=torch.int32)
