@@ -16,8 +16,9 @@
 // flight at a time, the first four while the token's sequence, page and angles are looked up.
 //
 // What bounds it is HBM: 8 x 4096 tokens of 32 / 32 heads with norms in 185 us (5.8 TB/s, where a plain copy of the same
-// bytes takes 168), an append of 2 x 8192 tokens of 32 / 8 heads in 74 us (5.4 TB/s; it looks up its page first).  Small
-// calls are bound by the launch: 2.5 to 3.4 us on the GPU, 3.6 to 5 us of host time.
+// bytes takes 168), an append of 2 x 8192 tokens of 32 / 8 heads in 74 us (5.4 TB/s; builds that skipped the look-up of the
+// page, and the angles, took 2 and 1 us less).  Small calls are bound by the launch: 2.5 to 3.4 us on the GPU, 3.3 to 5 us
+// of host time.
 #include "nb200_common.cuh"
 
 namespace nb200 {

@@ -1,6 +1,6 @@
 """CPU restatement, in 64 bits, of the operators around the paged KV cache (test infrastructure; see package docstring).
 
-The reference has none of them; the definitions are this build's own (parity unpinned).  A ragged batch: rows
+The reference has none of them, so the definitions here are the operators' own.  A ragged batch: rows
 cu[b] .. cu[b+1]-1 are the last tokens of sequence b, whose length with them is lens[b]; row t is at position
 lens[b] - cu[b+1] + t.  Page p of sequence b is pool page table[b, p]; a page holds 64 rows.
 """

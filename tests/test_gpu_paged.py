@@ -342,6 +342,17 @@ def test_chunk_attention_of_many_sequences(cuda, native_lib):
     check_attention(batch, q, out)
 
 
+def test_chunk_attention_over_shared_pages(cuda, native_lib):
+    """Sequences that begin with the same pages, and one that holds a page twice."""
+    batch = Batch([5, 70, 1], [300, 250, 200], 2, torch.bfloat16)
+    batch.table[1, :2] = batch.table[0, :2]
+    batch.table[2, :2] = batch.table[0, 0]
+    q = randn((batch.T, 6, D), 28, torch.bfloat16)
+    out = attend(batch, q.to(cuda), cuda)
+    finish()
+    check_attention(batch, q, out)
+
+
 def test_chunk_attention_with_strided_queries_and_output(cuda, native_lib):
     """Queries inside a packed projection, the output inside a wider buffer and head-major."""
     batch = Batch([50, 9], [90, 400], 2, torch.bfloat16)
