@@ -11,12 +11,15 @@ the kernel library every call raises.
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import native
 
 _TORCH_DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 _status_buffers: dict[int, torch.Tensor] = {}
+_status_lock = threading.Lock()
 
 
 def _check(name: str, t, shape, dtype: str | torch.dtype) -> None:
@@ -71,13 +74,20 @@ def _pools(k_pages, v_pages, Hkv: int, page_size: int, D: int, dtype: str) -> No
 
 
 def status_buffer(dev: torch.device) -> torch.Tensor:
-    """Per-device int32[4] that kernels with bounded device-side waits report into."""
+    """Per-device int32[4] that kernels with bounded device-side waits report into.
+
+    Made once per device, whichever threads ask first: the native binding keeps the address, so it must be that of the
+    tensor that stays.
+    """
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     buf = _status_buffers.get(idx)
     if buf is None:
-        buf = torch.zeros(native.STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status_buffers[idx] = buf
-        native.binding().set_status(idx, buf.data_ptr())
+        with _status_lock:
+            buf = _status_buffers.get(idx)
+            if buf is None:
+                buf = torch.zeros(native.STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
+                native.binding().set_status(idx, buf.data_ptr())
+                _status_buffers[idx] = buf
     return buf
 
 

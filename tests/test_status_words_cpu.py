@@ -1,0 +1,69 @@
+"""The per-device status words without a GPU: host memory stands in for the device's, a fake for the native binding."""
+
+import threading
+import time
+
+import pytest
+import torch
+
+from neptune_mlir import native, runtime
+
+DEVICE = torch.device("cuda", 0)
+
+
+class FakeBinding:
+    """Keeps the address that was published last, as the native binding does."""
+
+    def __init__(self, delays=()):
+        self.delays, self.published = list(delays), {}
+
+    def set_status(self, device, address):
+        time.sleep(self.delays.pop(0) if self.delays else 0.0)
+        self.published[device] = address
+
+
+@pytest.fixture
+def words(monkeypatch):
+    """Host tensors in the place of device ones, no capture running; returns a function that starts over."""
+    host_zeros = torch.zeros
+
+    class Stream:
+        def synchronize(self):
+            pass
+
+    def start(make_delays=(), publish_delays=()):
+        delays, binding = list(make_delays), FakeBinding(publish_delays)
+
+        def zeros(*args, device=None, **kwargs):
+            time.sleep(delays.pop(0) if delays else 0.0)
+            return host_zeros(*args, **kwargs)
+
+        monkeypatch.setattr(torch, "zeros", zeros)
+        monkeypatch.setattr(native, "binding", lambda: binding)
+        monkeypatch.setattr(runtime, "_status_buffers", {})
+        return binding
+
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    return start
+
+
+@pytest.mark.parametrize("make,publish", [((0.05, 0.15), (0.25, 0.0)), ((0.0, 0.0), (0.1, 0.0)), ((0.0,) * 2, (0.0,) * 2)])
+def test_first_calls_of_two_threads_publish_the_words_that_stay(words, make, publish):
+    """Whichever thread is first at each step, the binding ends with the address of the tensor that is kept."""
+    binding = words(make, publish)
+    together, got = threading.Barrier(2), []
+
+    def first_call():
+        together.wait()
+        runtime._first_status_buffer(DEVICE)
+        got.append(runtime.status_buffer(DEVICE).data_ptr())
+
+    threads = [threading.Thread(target=first_call) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    kept = runtime._status_buffers[0].data_ptr()
+    assert got == [kept, kept]
+    assert binding.published == {0: kept}
