@@ -19,6 +19,7 @@ from . import native
 
 _TORCH_DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 _status_buffers: dict[int, torch.Tensor] = {}
+_captured_words: dict[int, list[torch.Tensor]] = {}   # words of calls that were captured before the device had its own
 _status_lock = threading.Lock()
 
 
@@ -77,15 +78,20 @@ def status_buffer(dev: torch.device) -> torch.Tensor:
     """Per-device int32[4] that kernels with bounded device-side waits report into.
 
     Made once per device, whichever threads ask first: the native binding keeps the address, so it must be that of the
-    tensor that stays.
+    tensor that stays.  The stream that clears it is waited for, because every stream of the device uses it from then
+    on.  A graph capture cannot wait: words made inside one are that call's alone, cleared by each replay.
     """
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     buf = _status_buffers.get(idx)
     if buf is None:
-        with _status_lock:
+        with _status_lock, torch.cuda.device(idx):
             buf = _status_buffers.get(idx)
             if buf is None:
                 buf = torch.zeros(native.STATUS_WORDS, dtype=torch.int32, device=torch.device("cuda", idx))
+                if torch.cuda.is_current_stream_capturing():
+                    _captured_words.setdefault(idx, []).append(buf)
+                    return buf
+                torch.cuda.current_stream(idx).synchronize()
                 native.binding().set_status(idx, buf.data_ptr())
                 _status_buffers[idx] = buf
     return buf
@@ -94,11 +100,12 @@ def status_buffer(dev: torch.device) -> torch.Tensor:
 def check_status(device=None) -> None:
     """Synchronise and raise if a kernel reported an expired device-side wait on ``device``."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    buf = status_buffer(dev)
-    rc = native.lib().nb200_status_read(buf.data_ptr(), None, _stream(dev))
-    if rc != 0:
-        buf.zero_()
-    native.check(rc, "nb200 status")
+    own = status_buffer(dev)
+    for buf in (own, *_captured_words.get(own.device.index, ())):
+        rc = native.lib().nb200_status_read(buf.data_ptr(), None, _stream(dev))
+        if rc != 0:
+            buf.zero_()
+        native.check(rc, "nb200 status")
 
 
 def attn_fwd(q, k, v, out, *, shape, kv_len, dtype, scale_log2, causal) -> None:

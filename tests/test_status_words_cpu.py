@@ -1,5 +1,6 @@
 """The per-device status words without a GPU: host memory stands in for the device's, a fake for the native binding."""
 
+import contextlib
 import threading
 import time
 
@@ -26,13 +27,15 @@ class FakeBinding:
 def words(monkeypatch):
     """Host tensors in the place of device ones, no capture running; returns a function that starts over."""
     host_zeros = torch.zeros
+    waited = []
 
     class Stream:
         def synchronize(self):
-            pass
+            waited.append(dict(runtime._status_buffers))      # what could be seen before the words were clear
 
     def start(make_delays=(), publish_delays=()):
         delays, binding = list(make_delays), FakeBinding(publish_delays)
+        binding.waited = waited
 
         def zeros(*args, device=None, **kwargs):
             time.sleep(delays.pop(0) if delays else 0.0)
@@ -41,10 +44,13 @@ def words(monkeypatch):
         monkeypatch.setattr(torch, "zeros", zeros)
         monkeypatch.setattr(native, "binding", lambda: binding)
         monkeypatch.setattr(runtime, "_status_buffers", {})
+        monkeypatch.setattr(runtime, "_captured_words", {}, raising=False)
+        waited.clear()
         return binding
 
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
     return start
 
 
@@ -67,3 +73,26 @@ def test_first_calls_of_two_threads_publish_the_words_that_stay(words, make, pub
     kept = runtime._status_buffers[0].data_ptr()
     assert got == [kept, kept]
     assert binding.published == {0: kept}
+
+
+def test_the_words_are_clear_before_other_streams_can_use_them(words):
+    """The fill is asynchronous: its stream is waited for once, before anything of the words can be seen."""
+    binding = words()
+    runtime._first_status_buffer(DEVICE)
+    runtime.status_buffer(DEVICE)
+    assert binding.waited == [{}] and 0 in runtime._status_buffers
+
+
+def test_words_made_inside_a_capture_are_for_that_graph_alone(words, monkeypatch):
+    """Their fill is part of the graph, so no call outside it may take them for clear."""
+    binding = words()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    captured = runtime.status_buffer(DEVICE)
+    assert binding.waited == [] and binding.published == {} and runtime._status_buffers == {}
+    with pytest.raises(RuntimeError, match="before capturing"):
+        runtime._first_status_buffer(DEVICE)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    runtime._first_status_buffer(DEVICE)
+    kept = runtime.status_buffer(DEVICE)
+    assert kept.data_ptr() != captured.data_ptr() and binding.published == {0: kept.data_ptr()}
+    assert [w.data_ptr() for w in runtime._captured_words[0]] == [captured.data_ptr()]   # as long as the graph may run
