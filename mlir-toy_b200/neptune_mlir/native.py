@@ -111,7 +111,7 @@ def binding():
     global _BINDING
     if _BINDING is None:
         lib()
-        path = find_binding_path()
+        path = find_binding_path(_LIB_PATH)
         if path is None:
             raise NativeLibraryError("the torch binding (nb200_torch.so) was not found; build it with "
                                      "`python mlir-toy_b200/build_native.py`")

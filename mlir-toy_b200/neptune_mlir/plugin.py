@@ -67,9 +67,11 @@ def find_front_path(explicit: str | os.PathLike[str] | None = None) -> Path | No
     return _resolve(explicit, DEFAULT_FRONT_ENV, FRONT_PATTERNS)
 
 
-def find_binding_path() -> Path | None:
-    """Resolve nb200_torch.so (the CPython module between torch tensors and the kernel library) in the same directories."""
-    return next((m.resolve() for d in _candidate_dirs() if d.is_dir() and (m := _find_in_dir(d, BINDING_PATTERNS))), None)
+def find_binding_path(library: Path | None = None) -> Path | None:
+    """Resolve nb200_torch.so (the CPython module between torch tensors and the kernel library): beside ``library``, the
+    kernel library that was loaded, then in the same directories."""
+    directories = [*([library.parent] if library else []), *_candidate_dirs()]
+    return next((m.resolve() for d in directories if d.is_dir() and (m := _find_in_dir(d, BINDING_PATTERNS))), None)
 
 
 def find_plugin_path(explicit: str | os.PathLike[str] | None = None) -> Path | None:

@@ -77,8 +77,8 @@ def _pools(k_pages, v_pages, Hkv: int, page_size: int, D: int, dtype: str) -> No
 def status_buffer(dev: torch.device) -> torch.Tensor:
     """Per-device int32[4] that kernels with bounded device-side waits report into.
 
-    Made once per device, whichever threads ask first: the native binding keeps the address, so it must be that of the
-    tensor that stays.  The stream that clears it is waited for, because every stream of the device uses it from then
+    Made once per device, whichever threads ask first: the native binding keeps the address (_first_status_buffer), so
+    there is one tensor and it stays.  The stream that clears it is waited for, because every stream of the device uses it from then
     on.  A graph capture cannot wait: words made inside one are that call's alone, cleared by each replay.
     """
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
@@ -92,7 +92,6 @@ def status_buffer(dev: torch.device) -> torch.Tensor:
                     _captured_words.setdefault(idx, []).append(buf)
                     return buf
                 torch.cuda.current_stream(idx).synchronize()
-                native.binding().set_status(idx, buf.data_ptr())
                 _status_buffers[idx] = buf
     return buf
 
@@ -226,10 +225,11 @@ def _refuse(what: str):
 
 
 def _first_status_buffer(dev: torch.device) -> None:
-    """Make a device's status words; not inside a graph capture, whose memory ends with the graph."""
+    """Give the native binding the address of a device's status words, which are not made inside a graph capture: their
+    memory would end with the graph."""
     if dev.index not in _status_buffers and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("the first call on a device makes its status words: call once before capturing a graph")
-    status_buffer(dev)
+    native.binding().set_status(dev.index, status_buffer(dev).data_ptr())
 
 
 def _weight_checks(weights, D: int, dtype: str) -> list:

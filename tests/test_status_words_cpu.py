@@ -96,3 +96,41 @@ def test_words_made_inside_a_capture_are_for_that_graph_alone(words, monkeypatch
     kept = runtime.status_buffer(DEVICE)
     assert kept.data_ptr() != captured.data_ptr() and binding.published == {0: kept.data_ptr()}
     assert [w.data_ptr() for w in runtime._captured_words[0]] == [captured.data_ptr()]   # as long as the graph may run
+
+
+def test_operators_outside_the_binding_do_not_need_it(words, monkeypatch):
+    """Dense attention, decode, the peer merge and check_status take the words' address themselves."""
+    words()
+
+    def missing():
+        raise native.NativeLibraryError("the torch binding (nb200_torch.so) was not found")
+
+    monkeypatch.setattr(native, "binding", missing)
+    for _ in range(2):
+        assert runtime.status_buffer(DEVICE).tolist() == [0, 0, 0, 0]
+    with pytest.raises(native.NativeLibraryError, match="torch binding"):
+        runtime._first_status_buffer(DEVICE)
+
+
+def test_the_binding_hears_of_words_that_an_earlier_operator_made(words):
+    binding = words()
+    kept = runtime.status_buffer(DEVICE)
+    assert binding.published == {}
+    runtime._first_status_buffer(DEVICE)
+    assert binding.published == {0: kept.data_ptr()} and runtime.status_buffer(DEVICE) is kept
+
+
+def test_the_binding_is_found_beside_the_library_that_was_loaded(native_lib, tmp_path, monkeypatch):
+    """A library that the environment names, and its binding, can be anywhere."""
+    from neptune_mlir import plugin
+
+    monkeypatch.setattr(plugin, "_candidate_dirs", lambda: [tmp_path / "elsewhere"])
+    library = tmp_path / "libnb200.so"
+    library.write_bytes(b"")
+    monkeypatch.setenv(plugin.DEFAULT_LIBRARY_ENV, str(library))
+    assert plugin.find_library_path() == library.resolve()
+    assert plugin.find_binding_path(plugin.find_library_path()) is None
+    beside = tmp_path / "nb200_torch.so"
+    beside.write_bytes(b"")
+    assert plugin.find_binding_path(plugin.find_library_path()) == beside.resolve()
+    assert plugin.find_binding_path() is None
