@@ -88,28 +88,35 @@ def build_front(force: bool = False) -> Path:
 
 
 def build_binding(force: bool = False) -> Path:
-    """The CPython module that calls the kernel library with torch tensors: g++ against torch's headers and libraries."""
+    """The CPython module that calls the kernel library with torch tensors: g++ against torch's headers and libraries.
+
+    Built again when its command changes, which names torch's version and place and the interpreter's headers.
+    """
+    import sysconfig
+
+    import torch
+
     BINDING_OUT.parent.mkdir(parents=True, exist_ok=True)
+    OBJ_DIR.mkdir(exist_ok=True)
+    gxx = shutil.which("g++") or shutil.which("c++")
+    if gxx is None:
+        raise RuntimeError("g++ not found; the torch binding cannot be built")
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1]
+    cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DNB200_TORCH_VERSION="{torch.__version__}"',
+           f"-I{INCLUDE}", f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           f"-isystem{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(BINDING_OUT),
+           f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    record = OBJ_DIR / "nb200_torch.command.txt"
+    same = record.exists() and record.read_text() == "\n".join(cmd)
     newest = max(BINDING_SRC.stat().st_mtime, (INCLUDE / "nb200.h").stat().st_mtime)
-    if force or not BINDING_OUT.exists() or BINDING_OUT.stat().st_mtime < newest:
-        import sysconfig
-
-        import torch
-
-        gxx = shutil.which("g++") or shutil.which("c++")
-        if gxx is None:
-            raise RuntimeError("g++ not found; the torch binding cannot be built")
-        root = Path(torch.__file__).resolve().parent
-        cuda = Path(_nvcc()).resolve().parents[1]
-        cmd = [gxx, "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               f"-I{INCLUDE}", f"-isystem{root / 'include'}", f"-isystem{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
-               f"-isystem{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(BINDING_SRC), "-o", str(BINDING_OUT),
-               f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-Wl,--unresolved-symbols=ignore-all",
-               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    if force or not same or not BINDING_OUT.exists() or BINDING_OUT.stat().st_mtime < newest:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             BINDING_OUT.unlink(missing_ok=True)               # one of an older header must not be loaded in its place
             raise RuntimeError(f"g++ failed on {BINDING_SRC.name}:\n{res.stdout}\n{res.stderr}")
+        record.write_text("\n".join(cmd))
     return BINDING_OUT
 
 

@@ -216,4 +216,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "nb200_torch", "Calls of the nb20
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_nb200_torch(void) { return PyModule_Create(&g_module); }
+// torch_version: the version whose headers this was compiled against; the loader compares it with the one that runs.
+PyMODINIT_FUNC PyInit_nb200_torch(void) {
+  PyObject *module = PyModule_Create(&g_module);
+  if (module && PyModule_AddStringConstant(module, "torch_version", NB200_TORCH_VERSION) < 0) Py_CLEAR(module);
+  return module;
+}

@@ -115,11 +115,19 @@ def binding():
         if path is None:
             raise NativeLibraryError("the torch binding (nb200_torch.so) was not found; build it with "
                                      "`python mlir-toy_b200/build_native.py`")
-        import torch  # noqa: F401  (the libraries the module needs)
+        import torch  # the libraries the module needs
 
         loader = importlib.machinery.ExtensionFileLoader("nb200_torch", str(path))
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nb200_torch", loader))
-        loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("nb200_torch", loader))
+            loader.exec_module(module)
+        except ImportError as exc:                            # a symbol that this torch does not have, for one
+            raise NativeLibraryError(f"{path} does not load ({exc}); build it again with "
+                                     "`python mlir-toy_b200/build_native.py`") from exc
+        built_for = getattr(module, "torch_version", "of an unknown version")
+        if built_for != torch.__version__:
+            raise NativeLibraryError(f"{path} was built for torch {built_for}, this is torch "
+                                     f"{torch.__version__}; build it again with `python mlir-toy_b200/build_native.py`")
         _bind(module)
         _BINDING = module
     return _BINDING
