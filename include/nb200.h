@@ -74,9 +74,9 @@ int nb200_attn_fwd(const void *q, const void *k, const void *v, void *out,
  * NB200_ERR_BAD_ARG if a kernel refused device-side data (code 22: a block-table entry outside the page pool;
  * code 23: an appended row whose position its block-table row does not reach),
  * NB200_ERR_DEVICE_TIMEOUT for every other code (an expired bounded wait). host_out may be NULL.
- * A non-zero status[0] makes later attention and SSD launches that are given the same buffer return at once
- * without touching their outputs (codes 22 and 23, refused data, do not stop nb200_attn_paged), so read it (and zero it)
- * after synchronising whenever a result matters. */
+ * A recorded expired wait makes later attention and SSD launches that are given the same buffer return at once
+ * without touching their outputs, so read it (and zero it) after synchronising whenever a result matters.  Refused data
+ * (codes 22 and 23) stops nobody else; it stays recorded until it is read, or until an expired wait takes its place. */
 int nb200_status_read(const int *status, int *host_out, void *stream);
 
 /*

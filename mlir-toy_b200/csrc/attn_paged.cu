@@ -84,7 +84,7 @@ constexpr int kMaxCtas = 160;                   // CTAs that the workspace has r
 constexpr long long kWaveBytes = 1ll << 26;     // half of the L2
 constexpr int kTileUnits = 2;                   // what changing tiles costs (2 us), in blocks, on the line that is cut
 
-enum : int { kErrProducer = 41, kErrMma = 42, kErrSoftmax = 43, kErrEpilogue = 44, kErrTable = 22, kErrSlot = 23 };
+enum : int { kErrProducer = 41, kErrMma = 42, kErrSoftmax = 43, kErrEpilogue = 44 };
 
 // Part of a tile that one CTA works on.
 struct Segment {
@@ -148,11 +148,7 @@ constexpr int kSmemBytes = kOffShared + 1024 + static_cast<int>(sizeof(Shared));
 static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
 
 __device__ __forceinline__ void report(int *status, int code, int detail) {
-  if (status && atomicCAS(status, 0, code) == 0) {
-    status[1] = static_cast<int>(blockIdx.x);
-    status[2] = detail;
-    status[3] = static_cast<int>(threadIdx.x);
-  }
+  status_record(status, code, static_cast<int>(blockIdx.x), detail, static_cast<int>(threadIdx.x));
 }
 
 // Waits for a phase with a limit on the turns: about 2 s if every turn suspends the thread for its microsecond, at least
@@ -276,7 +272,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the joining kernel waits for this grid's end itself
   if (warp == 14 && lane == 0) {
     const int code = a.status ? *reinterpret_cast<volatile int *>(a.status) : 0;
-    sh->skip = (code != 0 && code != kErrTable && code != kErrSlot) ? 1 : 0;   // an expired wait, not refused data
+    sh->skip = status_stops(code) ? 1 : 0;
     a.owners[blockIdx.x].parts = 0;
   }
 
@@ -468,7 +464,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (page >= pages) return outside;
         const int e = table[page];
         if (e >= 0 && e < a.num_pages) return e * a.Hkv + kvh;
-        if (is_k) report(a.status, kErrTable, e);
+        if (is_k) report(a.status, kStatusBadPage, e);
         return outside;
       };
       bool ok = true;

@@ -79,11 +79,7 @@ struct Shared {
 constexpr int kSmemBytes = 6 * kTileBytes + 1024 + static_cast<int>(sizeof(Shared));
 
 __device__ __forceinline__ void report(int *status, int code, int detail) {
-  if (status && atomicCAS(status, 0, code) == 0) {
-    status[1] = static_cast<int>(blockIdx.x);
-    status[2] = detail;
-    status[3] = static_cast<int>(threadIdx.x);
-  }
+  status_record(status, code, static_cast<int>(blockIdx.x), detail, static_cast<int>(threadIdx.x));
 }
 
 struct Problem {
@@ -127,7 +123,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 
   if (threadIdx.x == 0) {
     sh->abort_flag = 0;
-    sh->skip = (status != nullptr && *reinterpret_cast<volatile int *>(status) != 0) ? 1 : 0;
+    sh->skip = (status != nullptr && status_stops(*reinterpret_cast<volatile int *>(status))) ? 1 : 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&sh->q_full[b]), 1);
       mbar_init(smem_u32(&sh->q_empty[b]), 1);

@@ -289,15 +289,13 @@ struct RingBarriers {
 constexpr int kChunkRows = 2 * kStageRows;   // dynamic deal: rows a CTA takes from its head's counter at a time
                                              // (64 to 256 measured within 1 % of each other from 32 K to 256 K rows; 512 is slower)
 
-// Codes the ring kernel records in status[0] (block, detail and thread follow in status[1..3]).
-enum : int { kErrDecodeWait = 21, kErrDecodeBadPage = 22 };
+// Code the ring kernel records in status[0], beside kStatusBadPage (block, detail and thread follow in status[1..3]).
+constexpr int kErrDecodeWait = 21;
+constexpr int kAbortBadPage = 2;   // in abort_flag: no wait expired, the producer met a page outside the pool
 
 __device__ __forceinline__ void decode_report(int *status, int code, int detail) {
-  if (status && atomicCAS(status, 0, code) == 0) {
-    status[1] = static_cast<int>(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z));
-    status[2] = detail;
-    status[3] = static_cast<int>(threadIdx.x);
-  }
+  status_record(status, code, static_cast<int>(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)), detail,
+                static_cast<int>(threadIdx.x));
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void *gsrc, uint32_t bytes, uint32_t bar) {
@@ -581,8 +579,8 @@ decode_splitk_ring_kernel(const uint16_t *__restrict__ q, const uint16_t *__rest
           if (page < 0 || page >= num_pages) {
             // a table entry outside the pool: no copy is issued from it; the consumers see the abort flag, the
             // partial is poisoned and the status words say which entry it was
-            decode_report(status, kErrDecodeBadPage, page);
-            *abort_flag = 1;
+            decode_report(status, kStatusBadPage, page);
+            *abort_flag = kAbortBadPage;
             break;
           }
           off = ((size_t)page * Hkv + hkv) * kStageRows * kHeadDim;
@@ -622,7 +620,7 @@ decode_splitk_ring_kernel(const uint16_t *__restrict__ q, const uint16_t *__rest
       const int st = it % kRingStages;
       ok = __all_sync(0xffffffffu, sm100::mbar_wait(b_full + 8 * st, (it / kRingStages) & 1, abort_flag));
       if (!ok) {
-        if (lane == 0) decode_report(status, kErrDecodeWait, 1000000 + it);   // no-op if the producer already said why
+        if (lane == 0 && *abort_flag != kAbortBadPage) decode_report(status, kErrDecodeWait, 1000000 + it);
         break;
       }
       const unsigned char *sk = ring + st * 2 * kStageBytes + (warp * (kPairs * 2) + half) * (kHeadDim * 2) + c * 16;

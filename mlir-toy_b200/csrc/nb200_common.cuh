@@ -32,6 +32,22 @@ int fail(int code, const char *fmt, ...);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// ---- status words (see nb200_status_read) ---------------------------------------------------
+// Device-side data that a kernel refused and went on without; every other code is an expired wait, after which the work
+// of later launches that share the words would rest on an incomplete result.
+enum : int { kStatusBadPage = 22, kStatusNoSlot = 23 };
+__device__ __forceinline__ bool status_refused(int code) { return code == kStatusBadPage || code == kStatusNoSlot; }
+__device__ __forceinline__ bool status_stops(int code) { return code != 0 && !status_refused(code); }
+// Records a code if none is there.  An expired wait takes the place of refused data: it is what stops others.
+__device__ __forceinline__ void status_record(int *status, int code, int block, int detail, int detail2) {
+  if (!status) return;
+  const int found = atomicCAS(status, 0, code);
+  if (found != 0 && (status_refused(code) || !status_refused(found) || atomicCAS(status, found, code) != found)) return;
+  status[1] = block;
+  status[2] = detail;
+  status[3] = detail2;
+}
+
 // ---- storage element traits ----------------------------------------------------------------
 template <int DT> struct Elem;
 template <> struct Elem<NB200_F16> {

@@ -31,8 +31,6 @@ constexpr int kMaxHalf = 128;          // rot <= 256
 constexpr int kPageRows = 64;
 constexpr int kCacheD = 128;
 
-enum : int { kErrTable = 22, kErrSlot = 23 };   // see nb200_status_read
-
 struct Strides {
   long long b, t, h;                   // batch, token, head, in elements
 };
@@ -83,11 +81,7 @@ template <int DT> __device__ __forceinline__ piece_t<DT> from_float(const float 
 }
 
 __device__ __forceinline__ void report(int *status, int code, int detail, int detail2) {
-  if (status && atomicCAS(status, 0, code) == 0) {
-    status[1] = static_cast<int>(blockIdx.x);
-    status[2] = detail;
-    status[3] = detail2;
-  }
+  status_record(status, code, static_cast<int>(blockIdx.x), detail, detail2);
 }
 
 // Sequence whose tokens include row t, or -1: one before the first entry of cu_seqlens [B + 1] above t, found 32 ways at
@@ -164,13 +158,13 @@ __global__ void __launch_bounds__(kThreads, DT == NB200_F32 ? 5 : 7) norm_rope_k
     if (t < first || t >= end) return;                    // cu_seqlens is not a running sum
     const long long p = static_cast<long long>(a.seq_lens[b]) - end + t;
     if (p < 0 || p >= static_cast<long long>(a.max_pages) * kPageRows) {
-      if (lane == 0 && chunk == 0) report(a.status, kErrSlot, t, static_cast<int>(p));
+      if (lane == 0 && chunk == 0) report(a.status, kStatusNoSlot, t, static_cast<int>(p));
       return;
     }
     pos = static_cast<int>(p);
     const int page = a.block_table[static_cast<long long>(b) * a.max_pages + pos / kPageRows];
     if (page < 0 || page >= a.num_pages) {
-      if (lane == 0 && chunk == 0) report(a.status, kErrTable, page, 0);
+      if (lane == 0 && chunk == 0) report(a.status, kStatusBadPage, page, 0);
       return;
     }
     slot_base = (static_cast<long long>(page) * a.Hkv * kPageRows + pos % kPageRows) * kCacheD;

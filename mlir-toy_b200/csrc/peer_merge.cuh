@@ -64,11 +64,8 @@ __device__ __forceinline__ bool wait_arrival(const Ptrs &peers, int rows, int wo
   const unsigned long long t0 = timer_ns();
   while (ld_acquire_sys(flag) != generation) {
     if (timer_ns() - t0 > static_cast<unsigned long long>(wait_ns)) {
-      if (status && atomicCAS(status, 0, kErrWait) == 0) {
-        status[1] = static_cast<int>(blockIdx.x);
-        status[2] = r;                             // the rank whose partial never arrived
-        status[3] = static_cast<int>(generation);
-      }
+      // detail: the rank whose partial never arrived
+      status_record(status, kErrWait, static_cast<int>(blockIdx.x), r, static_cast<int>(generation));
       return false;
     }
     __nanosleep(64);
