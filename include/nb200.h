@@ -312,7 +312,8 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  * At most 128 query heads to a kv head; T below 2^30, max_pages * page_size up to 2^30.  Two kernels: the second joins the
  * tiles that were worked on by more than one CTA, in an order that lengths alone decide, so that equal calls give equal
  * bits.  out shares no element with the other tensors.
- * A row that sees nothing (its position is negative) is 0; rows that belong to no sequence are not touched.  Cache rows
+ * A row that sees nothing (its position is negative) is 0, one whose visible scores are all -infinity is NaN, as its
+ * softmax is; rows that belong to no sequence are not touched.  Cache rows
  * at and beyond a sequence's length are not used, whatever they hold; a value that is infinite or NaN makes that column
  * of the rows that see it not finite, and reaches no other row.  A table entry outside [0, num_pages) is never
  * dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and

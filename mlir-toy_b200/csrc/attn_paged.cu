@@ -742,8 +742,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       mbar_arrive(b_lm_free + 8 * (n & 1));
       const float mf = fmaxf(lm0.x, lm1.x);   // the running maximum never decreases: the later one is the larger
       float l = (lm0.y == 0.f ? 0.f : lm0.y * ex2(lm0.x - mf)) + (lm1.y == 0.f ? 0.f : lm1.y * ex2(lm1.x - mf));
-      // no visible row (in this part): every weight was 0 and every V looked through, so O is 0
-      const bool empty = l == 0.f;
+      // A row that sees nothing is 0: every weight was 0 and every V looked through, so O is.  One that sees scores of -inf
+      // alone has l = 0 too, and 0 / 0 = NaN as the softmax of such a row is.
+      const bool empty = last_seen < 0;
       if (bad) l = __int_as_float(0x7fffffff);
       const float inv = slot >= 0 || (empty && !bad) ? 1.f : 1.f / l;
       const uint64_t inv2 = f2_pack(inv, inv);
@@ -1032,7 +1033,8 @@ template <int DT> __global__ void __launch_bounds__(kJoinWarps * 32) attn_paged_
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  // Every row of a tile that was cut sees something: the tile has two blocks or more, its tokens are at 128 positions at most.
+  const float inv = 1.f / l;
   uint4 *dst = a.out + static_cast<size_t>(own.tok0 + token_of(a, r)) * a.out_t + static_cast<size_t>(own.kvh * a.group + r - token_of(a, r) * a.group) * a.out_h;
   reinterpret_cast<uint2 *>(dst)[lane] = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
 }

@@ -1,0 +1,72 @@
+"""Chunk attention and append over the paged cache where rows, values and weights are at their limits.
+
+Bounds are those of the module with the operators' tests: a rounding to the storage type is off by half a step.
+"""
+
+import math
+
+import pytest
+import torch
+
+from gpu_util import finish
+from oracle import paged
+from test_gpu_paged import D, NAMES, PAGE, Batch, attend, close_to_attention, randn
+
+pytestmark = pytest.mark.gpu
+
+SCALE = 1 / math.sqrt(D)
+
+
+def cache_row(batch, b, j):
+    """Pool page and row of position j of sequence b."""
+    return batch.table[b, j // PAGE].long(), j % PAGE
+
+
+def definition(batch, q):
+    """The 64-bit definition; its score bound without the keys that are not finite."""
+    exact, spread, _ = paged.attn_paged(q, batch.k, batch.v, batch.table, batch.cu, batch.lens, SCALE)
+    tame = batch.k.clone()
+    tame[~tame.isfinite()] = 0
+    _, _, score = paged.attn_paged(q, tame, batch.v, batch.table, batch.cu, batch.lens, SCALE)
+    return exact, spread, score
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=NAMES.get)
+@pytest.mark.parametrize("Hq,Hkv,new,lens", [(4, 1, [3, 2], [3, 40]), (8, 2, [130, 1], [130, 300]), (4, 2, [140], [200])])
+def test_rows_whose_visible_scores_are_all_minus_infinity_are_nan(cuda, native_lib, dtype, Hq, Hkv, new, lens):
+    """The first sequence's first keys score -inf with every query: the rows that see no others are NaN, as the softmax of
+    such a row is and unlike rows that see nothing; the rows after them are as if those keys were not there."""
+    batch = Batch(new, lens, Hkv, dtype)
+    q = randn((batch.T, Hq, D), 61, dtype)
+    q[..., 7] = 1.0
+    blind = lens[0] - new[0] + 2                              # the first two new rows see such keys alone
+    for j in range(blind):
+        page, row = cache_row(batch, 0, j)
+        batch.k[page, :, row, 7] = float("-inf")
+    out = attend(batch, q.to(cuda), cuda)
+    finish()
+    out = out.cpu()
+    exact, spread, score = definition(batch, q)
+    assert bool(exact[:2].isnan().all()) and bool(exact[2:batch.cu[-1]].isfinite().all())
+    assert bool(out[:2].isnan().all())
+    part = slice(2, batch.cu[-1])
+    close_to_attention(out[part], exact[part], spread[part], score, max(lens), 6.0, dtype)
+
+
+def test_a_row_of_minus_infinities_over_a_long_cache_is_nan(cuda, native_lib):
+    """The same where a row's blocks are split over many CTAs and joined: in one sequence every key, in another all but
+    the keys of one page."""
+    lens = [9000, 9000, 5000]
+    batch = Batch([1, 1, 2], lens, 2, torch.bfloat16)
+    q = randn((batch.T, 8, D), 62, torch.bfloat16)
+    q[..., 7] = 1.0
+    for b, kept in ((0, None), (1, 70)):
+        for p in range((lens[b] + PAGE - 1) // PAGE):
+            if p != kept:
+                batch.k[batch.table[b, p], :, :min(PAGE, lens[b] - p * PAGE), 7] = float("-inf")
+    out = attend(batch, q.to(cuda), cuda)
+    finish()
+    out = out.cpu()
+    exact, spread, score = definition(batch, q)
+    assert bool(exact[0].isnan().all()) and bool(out[0].isnan().all())
+    close_to_attention(out[1:4], exact[1:4], spread[1:4], score, 9000, 6.0, torch.bfloat16)
