@@ -314,8 +314,9 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  * bits.  out shares no element with the other tensors.
  * A row that sees nothing (its position is negative) is 0, one whose visible scores are all -infinity is NaN, as its
  * softmax is; rows that belong to no sequence are not touched.  Cache rows
- * at and beyond a sequence's length are not used, whatever they hold; a value that is infinite or NaN makes that column
- * of the rows that see it not finite, and reaches no other row.  A table entry outside [0, num_pages) is never
+ * at and beyond a sequence's length are not used, whatever they hold; an infinite value makes that column of the
+ * rows that see it infinite (NaN beside one of the other sign, and it may where its weight rounds to 0), a NaN makes it
+ * NaN; neither reaches another row.  A table entry outside [0, num_pages) is never
  * dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and
  * `status` records code 22.
  */

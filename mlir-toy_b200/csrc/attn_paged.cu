@@ -46,7 +46,8 @@
 // may hold anything there.  V may not, since 0 * NaN is NaN: in the blocks that some row of the tile does not see
 // whole, the epilogue warps (idle then) clear V rows behind the sequence's end in shared memory, and look for infinities
 // and NaN in the rows that only some of the tile's rows see, before the PV product of that block.  Such a value is
-// replaced by 0 and noted; the epilogue makes it a NaN in exactly those rows that see it.
+// replaced by 0 and noted, and the epilogue adds it to that column of exactly those rows that see it, so that it gives
+// what the product gives in the other blocks: an infinity, or NaN beside one of the other sign.
 //
 // Every wait is bounded; on expiry the role records a code in the status words and unwinds.
 #include <cuda.h>
@@ -128,7 +129,7 @@ struct Shared {
   uint64_t o_full[4], o_free[4], m_ready[2], lm_ready[2], lm_free[2], notes_read;
   uint64_t look[2], looked[2];       // V of a block to be looked through is on its way / has been looked through, per stage
   uint64_t sched_full[kSched];
-  unsigned long long taint[2][kD];   // per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is not finite)
+  unsigned long long taint[2][3][kD];   // of NaN, inf, -inf per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is so)
   unsigned scan[kThreads / 32];
   int waves;                         // whole tiles that every CTA takes first
   unsigned base;                     // units of the tiles dealt out like that
@@ -217,6 +218,10 @@ template <int DT> __device__ __forceinline__ uint32_t finite_probe(uint32_t x, u
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(acc));
   return r;
 }
+// 0: NaN, 1: inf, 2: -inf, of a value that is not finite.
+template <int DT> __device__ __forceinline__ int kind16(uint32_t h) {
+  return (h & (DT == NB200_BF16 ? 0x7fu : 0x3ffu)) ? 0 : 1 + ((h >> 15) & 1);
+}
 template <int DT> __device__ __forceinline__ bool not_finite16(uint32_t h) {
   return DT == NB200_BF16 ? (h & 0x7f80u) == 0x7f80u : (h & 0x7c00u) == 0x7c00u;
 }
@@ -235,7 +240,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   Shared *sh = reinterpret_cast<Shared *>(smem + kOffShared);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x < 2 * kD) sh->taint[threadIdx.x / kD][threadIdx.x % kD] = 0;
+  for (int i = threadIdx.x; i < 2 * 3 * kD; i += kThreads) (&sh->taint[0][0][0])[i] = 0;
   if (warp == 15) {
     tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
     tmem_relinquish();
@@ -701,8 +706,9 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             for (int c = 0; c < kD; ++c) {   // column c: 16-byte piece (c / 8) % 8 of its half, swizzled with the row
               uint16_t *x = reinterpret_cast<uint16_t *>(row + (c >> 6) * kBox + (((c >> 3) ^ r) & 7) * 16) + (c & 7);
               if (not_finite16<DT>(*x)) {
+                const int kind = kind16<DT>(*x);
                 *x = 0;
-                atomicMax(&sh->taint[m & 1][c], (static_cast<unsigned long long>(m + 1) << 32) | (0x7fffffffu - static_cast<unsigned>(col0 + r)));
+                atomicMax(&sh->taint[m & 1][kind][c], (static_cast<unsigned long long>(m + 1) << 32) | (0x7fffffffu - static_cast<unsigned>(col0 + r)));
                 *reinterpret_cast<volatile int *>(&sh->taint_any[m & 1]) = m + 1;
               }
             }
@@ -797,17 +803,23 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           __syncwarp();
         }
       }
-      if (tainted) {   // columns whose values are not finite: NaN in the rows that see them
+      if (tainted) {   // columns with values that are not finite: added in the rows that see them
         __syncwarp();
         uint16_t *const mine = reinterpret_cast<uint16_t *>(dst + static_cast<size_t>(tok) * a.out_t + static_cast<size_t>(row - tok * a.group) * a.out_h);
 #pragma unroll 1
         for (int c = 0; c < kD && tok < ntok; ++c) {
-          const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][c]);
-          if (static_cast<int>(note >> 32) != n + 1 || static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) > last_seen) continue;
+          float add = 0.f;
+#pragma unroll 1
+          for (int kind = 0; kind < 3; ++kind) {
+            const unsigned long long note = *reinterpret_cast<volatile unsigned long long *>(&sh->taint[n & 1][kind][c]);
+            if (static_cast<int>(note >> 32) == n + 1 && static_cast<int>(0x7fffffffu - static_cast<uint32_t>(note)) <= last_seen)
+              add += __int_as_float(kind == 0 ? 0x7fffffff : (kind == 1 ? 0x7f800000 : 0xff800000));
+          }
+          if (add == 0.f) continue;
           if (slot < 0)
-            mine[c] = 0x7fffu;
+            store1<DT>(mine, c, load1<DT>(mine, c) + add);
           else
-            po[c] = __int_as_float(0x7fffffff);
+            po[c] += add;
         }
         __syncwarp();
         // every warp has read its notes before any looks on and writes over them

@@ -70,3 +70,35 @@ def test_a_row_of_minus_infinities_over_a_long_cache_is_nan(cuda, native_lib):
     exact, spread, score = definition(batch, q)
     assert bool(exact[0].isnan().all()) and bool(out[0].isnan().all())
     close_to_attention(out[1:4], exact[1:4], spread[1:4], score, 9000, 6.0, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=NAMES.get)
+@pytest.mark.parametrize("Hq,Hkv,new,lens", [(8, 2, [150, 4], [700, 300]), (4, 2, [6, 1], [9000, 50]), (24, 3, [16, 16], [131, 700])])
+def test_values_that_are_not_finite_are_added_wherever_they_stand(cuda, native_lib, dtype, Hq, Hkv, new, lens):
+    """Infinities of either sign and NaN, in blocks that every row of a tile sees and in those that only some do: a row
+    that sees them gets their sum, a row that does not is as if they were not there."""
+    batch = Batch(new, lens, Hkv, dtype)
+    q = randn((batch.T, Hq, D), 63, dtype)
+    start = lens[0] - new[0]
+    inf, nan, late = float("inf"), float("nan"), start + new[0] // 2
+    placed = [(0, 5, inf), (late, 6, inf), (late, 7, -inf), (1, 8, -inf), (late, 8, -inf), (1, 9, inf), (late, 9, -inf),
+              (late, 10, nan), (0, 11, nan), (late, 12, -inf), (lens[0] - 1, 12, inf), (lens[0] - 1, 127, -inf)]
+    exact_values = batch.v.clone()
+    for j, col, value in placed:
+        page, row = cache_row(batch, 0, j)
+        batch.v[page, 1, row, col] = value
+        exact_values[page, 1, row, col] = 0
+    out = attend(batch, q.to(cuda), cuda)
+    finish()
+    out, total = out.cpu(), batch.cu[-1]
+    exact, spread, score = paged.attn_paged(q, batch.k, exact_values, batch.table, batch.cu, batch.lens, SCALE)
+    group = Hq // Hkv
+    added = torch.zeros(exact.shape)
+    for j, col, value in placed:
+        added[max(0, j - start):new[0], group:2 * group, col] += value
+    seen = added[:total] != 0
+    assert int(seen.sum()) > 0
+    want = added[:total][seen]
+    assert torch.equal(out[:total][seen].float().nan_to_num(nan=1.0, posinf=2.0, neginf=3.0), want.nan_to_num(nan=1.0, posinf=2.0, neginf=3.0))
+    out = torch.where(added != 0, exact.to(dtype), out)
+    close_to_attention(out[:total], exact[:total], spread[:total], score, max(lens), 6.0, dtype)
