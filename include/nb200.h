@@ -266,7 +266,8 @@ int nb200_decode_fwd_static(const void *q, const void *k, const void *v, void *o
  *               addresses are multiples of 16 bytes.  So q and k may be views into a packed projection and q_out,
  *               k_out [B, H, S, D] tensors as nb200_attn_fwd reads them.
  * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.  An output's
- * rows lie apart: a stride smaller than a row is refused, unless its extent is 1.
+ * rows lie apart, and its dimensions nest: taken by size, a stride that does not cover what the smaller ones reach is refused,
+ * unless its extent is 1.
  */
 int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, void *k_out, const int *positions,
                        const float *inv_freq, const void *q_weight, const void *k_weight, const long long *strides,
@@ -306,8 +307,8 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  *   q, out [T, Hq, D]   (f16 or bf16, D == 128, Hq % Hkv == 0)   pools, table, cu_seqlens, seq_lens as above
  *   workspace  : nb200_attn_paged_workspace_bytes() bytes, 16-byte aligned, need not be cleared.  Calls that can overlap
  *                on the GPU need one each.
- *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out: multiples of 16 bytes, at least a row (the
- *                stride of an extent of 1 is not used)
+ *   strides    : HOST array of 4: the token and head stride (in elements) of q and of out: multiples of 16 bytes, at least a row,
+ *                out's rows apart as for nb200_qk_norm_rope (the stride of an extent of 1 is not used)
  *   scale_log2 : log2(e) * softmax scale
  * At most 128 query heads to a kv head; T below 2^30, max_pages * page_size up to 2^30.  Two kernels: the second joins the
  * tiles that were worked on by more than one CTA, in an order that lengths alone decide, so that equal calls give equal

@@ -30,6 +30,26 @@ int fail(int code, const char *fmt, ...);
     if (!(cond)) return ::nb200::fail(code, __VA_ARGS__);                                        \
   } while (0)
 
+// Whether the rows of `row` elements of a tensor with these extents and strides lie apart, for a layout whose dimensions nest:
+// taken by size, each stride covers all that the ones below it reach.  Strides of extents of 1 are not used.
+template <int N> inline bool rows_apart(int row, const long long (&extents)[N], const long long (&strides)[N]) {
+  double covered = row;                                  // elements up to the end of the last row, so far
+  bool used[N] = {};
+  for (int n = 0; n < N; ++n) {
+    int least = -1;
+    double size = 0;
+    for (int i = 0; i < N; ++i) {
+      const double s = strides[i] < 0 ? -static_cast<double>(strides[i]) : static_cast<double>(strides[i]);
+      if (!used[i] && extents[i] > 1 && (least < 0 || s < size)) least = i, size = s;
+    }
+    if (least < 0) break;
+    if (size < covered) return false;
+    used[least] = true;
+    covered += size * static_cast<double>(extents[least] - 1);
+  }
+  return true;
+}
+
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- status words (see nb200_status_read) ---------------------------------------------------

@@ -325,6 +325,7 @@ int check_rows_apart(const char *who, const char *name, const Strides &s, int B,
   auto apart = [&](int extent, long long stride) { return extent == 1 || stride >= D || stride <= -D; };
   NB200_REQUIRE(apart(B, s.b) && apart(S, s.t) && apart(H, s.h), NB200_ERR_BAD_ARG,
                 "%s: the strides of %s must be at least a row", who, name);
+  NB200_REQUIRE(rows_apart(D, {B, S, H}, {s.b, s.t, s.h}), NB200_ERR_BAD_ARG, "%s: the rows of %s must lie apart", who, name);
   return NB200_OK;
 }
 int check_rotation(const char *who, int D, int rot, float eps) {

@@ -158,3 +158,27 @@ def test_the_oracle_rotates_a_pair_by_its_angle():
         torch.testing.assert_close(dots[0], dots[1])
         y, _ = paged.norm_rope(x, torch.ones(32), torch.tensor([0, 0]), freq, 0.0, interleaved)
         torch.testing.assert_close(y.pow(2).mean(-1), torch.ones((2, 1), dtype=torch.float64))
+
+
+def test_outputs_whose_rows_coincide_only_together_are_refused(native_lib, ptr):
+    """Strides that are each a row or more, and of which two, or one and a multiple of another, are the same address."""
+    lib, p = native.load(str(native_lib)), ptr[0]
+
+    def norm_rope(q_out, B=2, S=8):
+        strides = longs(2048, 256, 128, 2048, 256, 128, *q_out, 2048, 256, 128, 0)
+        return lib.nb200_qk_norm_rope(p, p, p, p, p, p, None, None, strides, B, S, 2, 2, 128, 128, 0, 1e-6, 1, None)
+
+    def append(q_out, Hq=2):
+        strides = longs(128 * Hq, 128, 256, 128, 256, 128, *q_out)
+        return lib.nb200_rope_append(p, p, p, p, p, p, p, p, p, p, None, None, strides, 2, 1, Hq, 2, 8, 4, 64, 128, 128, 0,
+                                     1e-6, 1, None, None)
+
+    def attend(out, T=2):
+        return lib.nb200_attn_paged(p, p, p, p, p, p, p, p, longs(512, 128, *out), T, 1, 4, 2, 8, 4, 64, 128, 1, 0.1, None, None)
+
+    for call, out, name in ((norm_rope, (128, 128, 128), b"q_out"), (norm_rope, (2048, 128, 128), b"q_out"),
+                            (norm_rope, (256, 256, 128), b"q_out"), (norm_rope, (1024, 256, -128), b"q_out"),
+                            (norm_rope, (2048, 256, 2048), b"q_out"), (norm_rope, (1024, 128, 896), b"q_out"),
+                            (append, (128, 128), b"q_out"), (append, (256, 256), b"q_out"), (append, (200, 128), b"q_out"),
+                            (attend, (128, 128), b"out"), (attend, (384, 128), b"out"), (attend, (136, 256), b"out")):
+        assert call(out) == -1 and b"rows of " + name + b" must lie apart" in lib.nb200_last_error(), (call, out, lib.nb200_last_error())
