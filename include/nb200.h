@@ -263,7 +263,8 @@ int nb200_decode_fwd_static(const void *q, const void *k, const void *v, void *o
  *   positions : int32 [B, S] (any value, negative ones too)
  *   strides   : HOST array of 13: the batch, token and head stride (in elements) of q, k, q_out and k_out in this order,
  *               then the batch stride of positions (0: one row for all).  Rows are contiguous; strides and base
- *               addresses are multiples of 16 bytes.  So q and k may be views into a packed projection and q_out,
+ *               addresses are multiples of 16 bytes, but for the batch or token stride of an extent of 1, which is not
+ *               used.  So q and k may be views into a packed projection and q_out,
  *               k_out [B, H, S, D] tensors as nb200_attn_fwd reads them.
  * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.  An output's
  * rows lie apart, and its dimensions nest: taken by size, a stride that does not cover what the smaller ones reach is refused,

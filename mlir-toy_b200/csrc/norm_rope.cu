@@ -314,9 +314,10 @@ template <int DT> int launch_dense(const Args &a, long long tokens, cudaStream_t
   return launch_g<DT, 32, false>(a, tokens, rows, st);
 }
 
-int check_view(const char *who, const char *name, const void *p, const Strides &s, int size) {
+int check_view(const char *who, const char *name, const void *p, const Strides &s, int B, int S, int size) {
+  auto fits = [&](int extent, long long stride) { return extent == 1 || stride * size % 16 == 0; };   // one that is taken
   NB200_REQUIRE(aligned16(p), NB200_ERR_BAD_ARG, "%s: %s must be 16-byte aligned", who, name);
-  NB200_REQUIRE(s.b * size % 16 == 0 && s.t * size % 16 == 0 && s.h * size % 16 == 0, NB200_ERR_BAD_ARG,
+  NB200_REQUIRE(fits(B, s.b) && fits(S, s.t) && s.h * size % 16 == 0, NB200_ERR_BAD_ARG,
                 "%s: the strides of %s must be multiples of 16 bytes", who, name);
   return NB200_OK;
 }
@@ -360,8 +361,9 @@ extern "C" int nb200_qk_norm_rope(const void *q, const void *k, void *q_out, voi
   const char *const names[4] = {"q", "k", "q_out", "k_out"};
   for (int i = 0; i < 4; ++i) {
     *views[i] = Strides{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]};
-    if ((rc = check_view(who, names[i], ptrs[i], *views[i], size)) != NB200_OK) return rc;
-    if (i >= 2 && (rc = check_rows_apart(who, names[i], *views[i], B, S, i == 2 ? Hq : Hkv, D)) != NB200_OK) return rc;
+    const int H = i % 2 == 0 ? Hq : Hkv;
+    if ((rc = check_view(who, names[i], ptrs[i], *views[i], B, S, size)) != NB200_OK) return rc;
+    if (i >= 2 && (rc = check_rows_apart(who, names[i], *views[i], B, S, H, D)) != NB200_OK) return rc;
   }
   NB200_REQUIRE((!q_weight || aligned16(q_weight)) && (!k_weight || aligned16(k_weight)), NB200_ERR_BAD_ARG,
                 "%s: the weights must be 16-byte aligned", who);
@@ -402,7 +404,7 @@ extern "C" int nb200_rope_append(const void *q, const void *k, const void *v, vo
   for (int i = 0; i < 4; ++i) {
     if (Hq == 0 && (i == 0 || i == 3)) continue;
     *views[i] = Strides{0, strides[2 * i], strides[2 * i + 1]};
-    if ((rc = check_view(who, names[i], ptrs[i], *views[i], 2)) != NB200_OK) return rc;
+    if ((rc = check_view(who, names[i], ptrs[i], *views[i], 1, T, 2)) != NB200_OK) return rc;
     if (i == 3 && (rc = check_rows_apart(who, names[i], *views[i], 1, T, Hq, D)) != NB200_OK) return rc;
   }
   NB200_REQUIRE(aligned16(k_pages) && aligned16(v_pages), NB200_ERR_BAD_ARG, "%s: the page pools must be 16-byte aligned", who);

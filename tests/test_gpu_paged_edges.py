@@ -10,7 +10,7 @@ import torch
 
 from gpu_util import finish
 from oracle import paged
-from test_gpu_paged import D, NAMES, PAGE, Batch, attend, close_to_attention, randn
+from test_gpu_paged import D, NAMES, PAGE, Batch, attend, close_to_attention, close_to_rotation, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,35 @@ def test_values_that_are_not_finite_are_added_wherever_they_stand(cuda, native_l
     assert torch.equal(out[:total][seen].float().nan_to_num(nan=1.0, posinf=2.0, neginf=3.0), want.nan_to_num(nan=1.0, posinf=2.0, neginf=3.0))
     out = torch.where(added != 0, exact.to(dtype), out)
     close_to_attention(out[:total], exact[:total], spread[:total], score, max(lens), 6.0, dtype)
+
+
+def test_odd_strides_of_extents_of_one(cuda, native_lib):
+    """A batch of one and a step of one token, cut out of tensors whose other rows begin anywhere."""
+    from neptune_mlir import runtime
+
+    S, H, dtype = 9, 3, torch.bfloat16
+    freq = (10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float32) / D)).to(cuda)
+    x = randn((1, S, H, D), 71, dtype)
+    at = torch.arange(5, 5 + S, dtype=torch.int32)
+
+    def cut(t):                                               # the same elements, the stride of extent 1 odd
+        return t.contiguous().as_strided(t.shape, [7 if n == 1 else s for n, s in zip(t.shape, t.contiguous().stride())])
+
+    xd = cut(x.to(cuda))
+    q_out, k_out = (cut(torch.full((1, H, S, D), 7.0, dtype=dtype, device=cuda)) for _ in range(2))
+    runtime.qk_norm_rope(xd, xd, at.to(cuda), freq, q_out, k_out, B=1, S=S, Hq=H, Hkv=H, D=D, rot_dim=D, interleaved=False,
+                         eps=1e-6, dtype="bf16")
+    batch = Batch([1], [70], H, dtype, pad=0)
+    kp, vp = batch.k.to(cuda), batch.v.to(cuda)
+    one, one_out = cut(x[0, :1].to(cuda)), cut(torch.full((1, H, D), 7.0, dtype=dtype, device=cuda))
+    runtime.rope_append(one, one, one, kp, vp, *batch.device_args(cuda), freq, one_out, rot_dim=D, interleaved=False, eps=1e-6,
+                        **batch.facts(H))
+    finish()
+    exact, size = paged.norm_rope(x[0], None, at, freq.cpu(), 1e-6, False)
+    for out in (q_out, k_out):
+        close_to_rotation(out[0].transpose(0, 1), exact, size, dtype)
+    exact, size = paged.norm_rope(x[0, :1], None, torch.tensor([69]), freq.cpu(), 1e-6, False)
+    page, row = cache_row(batch, 0, 69)
+    close_to_rotation(one_out, exact, size, dtype)
+    close_to_rotation(kp.cpu()[page, :, row][None], exact, size, dtype)
+    assert torch.equal(vp.cpu()[page, :, row], x[0, 0])

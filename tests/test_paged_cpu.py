@@ -182,3 +182,16 @@ def test_outputs_whose_rows_coincide_only_together_are_refused(native_lib, ptr):
                             (append, (128, 128), b"q_out"), (append, (256, 256), b"q_out"), (append, (200, 128), b"q_out"),
                             (attend, (128, 128), b"out"), (attend, (384, 128), b"out"), (attend, (136, 256), b"out")):
         assert call(out) == -1 and b"rows of " + name + b" must lie apart" in lib.nb200_last_error(), (call, out, lib.nb200_last_error())
+
+
+def test_the_batch_or_token_stride_of_an_extent_of_one_is_not_looked_at(native_lib, ptr):
+    """It is never taken, whatever a slice of a wider tensor left there.  (A check that comes later refuses these calls.)"""
+    lib, p = native.load(str(native_lib)), ptr[0]
+    for strides, extents in (((1001, 128, 128), (1, 8, 1)), ((1024, 3, 128), (2, 1, 1)), ((1, 1, 128), (1, 1, 2))):
+        B, S, H = extents
+        rc = lib.nb200_qk_norm_rope(p, p, p, p, p, p, p + 4, None, longs(*strides * 4, 0), B, S, H, H, 128, 128, 0, 1e-6, 1, None)
+        assert rc == -1 and b"weights must be" in lib.nb200_last_error(), (strides, lib.nb200_last_error())
+    for strides, T, H in (((77, 128), 1, 2), ((0, 128), 1, 1), ((-3, 256), 1, 4)):
+        rc = lib.nb200_rope_append(p, p, p, p, p + 8, p, p, p, p, p, None, None, longs(*strides * 4), T, 1, H, H, 8, 4, 64, 128,
+                                   128, 0, 1e-6, 1, None, None)
+        assert rc == -1 and b"page pools" in lib.nb200_last_error(), (strides, lib.nb200_last_error())
