@@ -140,6 +140,7 @@ struct Shared {
   int taint_any[2];                  // tile number + 1
   uint32_t tmem_base;
   int skip;
+  int k_issued;                      // K blocks asked for: whoever waits for a whole tile sees that it goes on
   float mslot[2][kBM];               // running maximum decided by block g, slot g & 1
   float2 lm[2][2][kBM];              // of tile n in [n & 1], per warpgroup: (maximum last used, partial row sum)
 };
@@ -254,6 +255,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     sh->before = sh->units = sh->base = 0;
     sh->waves = 0;
     sh->taint_any[0] = sh->taint_any[1] = 0;
+    sh->k_issued = 0;
   }
   if (warp == 13) {
     // one barrier per lane and turn
@@ -514,6 +516,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
                 tma_load_3d(dst + kBox, tm, 64, 0, s0, bar);
                 tma_load_3d(dst + kBox + kPageBox, tm, 64, 0, s1, bar);
                 ++issued;
+                if (is_k) *const_cast<volatile int *>(&sh->k_issued) = issued;
                 if (!is_k && j >= check) mbar_arrive(b_look + 8 * st);   // PV(g-2) is done: v_full is at V(g)'s phase
               }
             }
@@ -664,7 +667,11 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       if (!ok || !seg->more) break;
       const int nblk = seg->nblk;
       if (n > 0) map = next_regions(map, g0);
-      const volatile Segment *after = segment_at(n + 1);
+      // Listed when tile n's last K block has been asked for, which may take longer than a wait lasts (4 s for 2^29 cached
+      // rows): as long as blocks are being asked for, the wait begins again.
+      const volatile Segment *after = nullptr;
+      for (int then = -1, now; after == nullptr && (now = *const_cast<volatile int *>(&sh->k_issued)) != then; then = now)
+        after = segment_at(n + 1);
       ok = __all_sync(0xffffffffu, after != nullptr);
       if (!ok) break;
       const int early = after->more ? min(after->nblk, 2) : 0;

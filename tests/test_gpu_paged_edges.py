@@ -134,3 +134,26 @@ def test_odd_strides_of_extents_of_one(cuda, native_lib):
     close_to_rotation(one_out, exact, size, dtype)
     close_to_rotation(kp.cpu()[page, :, row][None], exact, size, dtype)
     assert torch.equal(vp.cpu()[page, :, row], x[0, 0])
+
+
+def test_a_tile_that_takes_longer_than_a_wait_lasts(cuda, native_lib):
+    """2^29 cached rows of one sequence, its pages all the same one, a kv head to every SM: each tile takes some seconds,
+    more than the two of a bounded wait.  Every score is 0 and one value row in 64 is 1, so that sums are whole numbers
+    below 2^24 (values) and multiples of 128 below 2^31 (weights): the output is 1/64 exactly."""
+    from neptune_mlir import runtime
+
+    heads = torch.cuda.get_device_properties(cuda).multi_processor_count
+    rows = 2 ** 29
+    k = torch.zeros((1, heads, PAGE, D), dtype=torch.bfloat16, device=cuda)
+    v = torch.zeros_like(k)
+    v[:, :, 5] = 1.0
+    table = torch.zeros((1, rows // PAGE), dtype=torch.int32, device=cuda)
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([0, 1], [rows]))
+    q = torch.zeros((1, heads, D), dtype=torch.bfloat16, device=cuda)
+    out = torch.full_like(q, 7.0)
+    work = torch.empty(runtime.attn_paged_workspace_bytes(), dtype=torch.uint8, device=cuda)
+    finish()
+    runtime.attn_paged(q, k, v, table, cu, lens, work, out, T=1, B=1, Hq=heads, Hkv=heads, max_pages=rows // PAGE, page_size=PAGE,
+                       D=D, dtype="bf16", scale_log2=SCALE * math.log2(math.e))
+    finish()
+    assert bool((out == 1 / 64).all())
