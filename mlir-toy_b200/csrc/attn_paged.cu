@@ -129,7 +129,7 @@ struct Shared {
   uint64_t o_full[4], o_free[4], m_ready[2], lm_ready[2], lm_free[2], notes_read;
   uint64_t look[2], looked[2];       // V of a block to be looked through is on its way / has been looked through, per stage
   uint64_t sched_full[kSched];
-  unsigned long long taint[2][3][kD];   // of NaN, inf, -inf per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is so)
+  alignas(16) unsigned long long taint[2][3][kD];   // of NaN, inf, -inf per column: (tile number + 1) << 32 | (2^31 - 1 - first KV row that is so)
   unsigned scan[kThreads / 32];
   int waves;                         // whole tiles that every CTA takes first
   unsigned base;                     // units of the tiles dealt out like that
@@ -241,7 +241,8 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
   Shared *sh = reinterpret_cast<Shared *>(smem + kOffShared);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  for (int i = threadIdx.x; i < 2 * 3 * kD; i += kThreads) (&sh->taint[0][0][0])[i] = 0;
+  static_assert(sizeof(sh->taint) <= kThreads * sizeof(uint4), "one store per thread");
+  if (threadIdx.x < sizeof(sh->taint) / sizeof(uint4)) reinterpret_cast<uint4 *>(sh->taint)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
   if (warp == 15) {
     tmem_alloc(smem_u32(&sh->tmem_base), kTmemCols);
     tmem_relinquish();
