@@ -39,7 +39,8 @@
 //
 // P is rounded to the storage type because the second product takes both operands in one 16-bit type; the row sum adds
 // the unrounded values.  The running maximum passes between the warpgroups through shared memory, O is rescaled only when
-// it grows by more than 2^8 (a weight is then at most 2^8, far inside fp16).
+// it grows by more than 2^8.  A weight is then at most 2^8; in fp16 all are taken times 2^7 (at most 2^15, of 2^16), so that
+// the least that is not 0 is 2^-32 of the maximum's, not 2^-25: a long cache has many small ones.
 //
 // What is masked.  A table entry that is not needed or not in the pool becomes a coordinate outside the tensor map, which
 // TMA fills with zeros; nothing outside the pool is addressed.  Scores of hidden columns are replaced, not added to, so K
@@ -75,6 +76,7 @@ constexpr int kPageBox = kPageRows * 128;       // one page's half: 8 KB
 constexpr int kSBufs = 3;
 constexpr int kTmemCols = 512;                  // four regions of 128 columns
 constexpr float kRescaleThreshold = 8.0f;
+template <int DT> constexpr float kLift = DT == NB200_F16 ? 7.0f : 0.0f;   // weights are held times 2^kLift, in P, in O and in l
 constexpr int kSched = 16;                      // ring of tile descriptors handed from the K producer to the other roles
 constexpr int kMaxCtas = 160;                   // CTAs that the workspace has room for
 // Cut like that, the CTAs of a head are all over its K and V at any time, which is fine while those stay in the L2.  A
@@ -958,7 +960,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         }
         // ---- p = 2^(s*scale - m), row sum, pack to 16 bit; P overwrites columns 0..63 of S ----
         const float m_use = m_new == -INFINITY ? 0.f : m_new;    // nothing seen so far: every p is 2^(-inf) = 0
-        const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(-m_use, -m_use);
+        const uint64_t c2 = f2_pack(a.scale_log2, a.scale_log2), nm2 = f2_pack(kLift<DT> - m_use, kLift<DT> - m_use);
         uint64_t lsum2 = f2_pack(0.f, 0.f);
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {

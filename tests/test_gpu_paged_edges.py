@@ -157,3 +157,33 @@ def test_a_tile_that_takes_longer_than_a_wait_lasts(cuda, native_lib):
                        D=D, dtype="bf16", scale_log2=SCALE * math.log2(math.e))
     finish()
     assert bool((out == 1 / 64).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=NAMES.get)
+def test_many_small_weights_beside_a_large_one(cuda, native_lib, dtype):
+    """One key of weight 1 whose value is 0 and 2^16 - 1 keys of weight 2^-26 whose value is 1: a thousandth, all
+    of it from weights that are below half of fp16's least.  The rows of a head are not split (a kv head to every SM).
+    Weights of fp16 are held times 2^7, so that one is off by 2^-25 / 2^7 at most."""
+    from neptune_mlir import runtime
+
+    heads = torch.cuda.get_device_properties(cuda).multi_processor_count
+    rows = 2 ** 16
+    k = torch.zeros((2, heads, PAGE, D), dtype=dtype)
+    v = torch.ones_like(k)
+    k[0, :, 3, 0] = 26 / (16 * SCALE * math.log2(math.e))     # rounded to the type, as the definition takes it
+    v[0, :, 3] = 0
+    table = torch.ones((1, rows // PAGE), dtype=torch.int32)
+    table[0, 100] = 0
+    q = torch.zeros((1, heads, D), dtype=dtype)
+    q[..., 0] = 16
+    out = torch.full_like(q, 7.0).to(cuda)
+    work = torch.empty(runtime.attn_paged_workspace_bytes(), dtype=torch.uint8, device=cuda)
+    cu, lens = (torch.tensor(x, dtype=torch.int32, device=cuda) for x in ([0, 1], [rows]))
+    runtime.attn_paged(q.to(cuda), k.to(cuda), v.to(cuda), table.to(cuda), cu, lens, work, out, T=1, B=1, Hq=heads, Hkv=heads,
+                       max_pages=rows // PAGE, page_size=PAGE, D=D, dtype=NAMES[dtype], scale_log2=SCALE * math.log2(math.e))
+    finish()
+    exact, spread, score = paged.attn_paged(q[:, :1], k[:, :1], v[:, :1], table, [0, 1], [rows], SCALE)
+    assert 7e-4 < exact[0, 0, 0].item() < 1.3e-3
+    h, u = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    bound = h * exact.abs() + (h + 512 * u * score + 2 * rows * u) * spread + rows * 2.0 ** -32 * (dtype == torch.float16)
+    assert bool(((out.double().cpu() - exact).abs() <= bound).all()), (out[0, 0, 0].item(), exact[0, 0, 0].item(), bound.max().item())
