@@ -82,6 +82,37 @@ __device__ __forceinline__ void report(int *status, int code, int detail) {
   status_record(status, code, static_cast<int>(blockIdx.x), detail, static_cast<int>(threadIdx.x));
 }
 
+// Polling wait (mbarrier.test_wait never suspends the thread): the waiter continues a few cycles after the phase
+// completes instead of the 200-300 a suspended thread takes to come back.  For the single issuing thread only.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_poll(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+#pragma unroll 1
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (mbar_test_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      *abort_flag = 1;
+      return false;
+    }
+  }
+}
+
 struct Problem {
   int Sq, Skv, n_qtiles, n_units, group, causal, total;
 };
