@@ -1066,7 +1066,7 @@ int map_3d(CUtensorMap *tm, const void *ptr, const cuuint64_t (&dims)[3], const 
   EncodeTiledFnT enc = tma_encode_fn();
   NB200_REQUIRE(enc, NB200_ERR_LAUNCH, "attn_paged: cuTensorMapEncodeTiled is not available from the driver");
   const cuuint32_t estr[3] = {1, 1, 1};
-  const CUresult r = enc(tm, dtype == NB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+  const CUresult r = tma_encode(enc, tm, dtype == NB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   NB200_REQUIRE(r == CUDA_SUCCESS, NB200_ERR_LAUNCH, "attn_paged: cuTensorMapEncodeTiled failed with code %d", (int)r);

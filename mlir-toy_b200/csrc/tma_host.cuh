@@ -25,6 +25,14 @@ inline EncodeTiledFnT tma_encode_fn() {
   return fn;
 }
 
+// The driver wants a current context, which a thread whose first call this is does not have yet: the runtime gives it one.
+template <typename... A> inline CUresult tma_encode(EncodeTiledFnT enc, A... args) {
+  const CUresult r = enc(args...);
+  int dev = 0;
+  if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return r;
+  return enc(args...);
+}
+
 // Row-major [rows, cols] tensor of 16-bit elements; boxes of box_rows x 64 columns (128 bytes), 128-byte swizzle.
 inline int tma_map_2d_sw128(CUtensorMap *tm, const void *ptr, long long rows, long long cols, int dtype, int box_rows,
                             const char *who) {
@@ -34,7 +42,7 @@ inline int tma_map_2d_sw128(CUtensorMap *tm, const void *ptr, long long rows, lo
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 2};
   const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = enc(tm, dtype == NB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+  const CUresult r = tma_encode(enc, tm, dtype == NB200_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                          2, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -51,7 +59,7 @@ inline int tma_map_2d_f32(CUtensorMap *tm, const void *ptr, long long rows, long
   const cuuint64_t strides[1] = {static_cast<cuuint64_t>(cols) * 4};
   const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows)};
   const cuuint32_t estr[2] = {1, 1};
-  const CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(ptr), dims, strides, box, estr,
+  const CUresult r = tma_encode(enc, tm, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(ptr), dims, strides, box, estr,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   NB200_REQUIRE(r == CUDA_SUCCESS, NB200_ERR_LAUNCH, "%s: cuTensorMapEncodeTiled failed with code %d", who, (int)r);
