@@ -187,3 +187,128 @@ def test_many_small_weights_beside_a_large_one(cuda, native_lib, dtype):
     h, u = torch.finfo(dtype).eps / 2, 2.0 ** -24
     bound = h * exact.abs() + (h + 512 * u * score + 2 * rows * u) * spread + rows * 2.0 ** -32 * (dtype == torch.float16)
     assert bool(((out.double().cpu() - exact).abs() <= bound).all()), (out[0, 0, 0].item(), exact[0, 0, 0].item(), bound.max().item())
+
+
+@pytest.mark.parametrize("B,prompt,cached,dtype", [(17, 5000, 300, torch.bfloat16), (40, 3001, 0, torch.float16),
+                                                   (300, 4096, 1000, torch.bfloat16), (512, 2500, 129, torch.float16)])
+def test_a_long_prompt_among_many_sequences(cuda, native_lib, B, prompt, cached, dtype):
+    """More sequences than a block has warps, one of them with a prompt of several thousand tokens: its place among the
+    others varies."""
+    at = (7 * B) % B if B % 2 else B // 2
+    new = [prompt if b == at else b % 2 for b in range(B)]
+    lens = [prompt + cached if b == at else new[b] + (37 * b) % 400 for b in range(B)]
+    batch = Batch(new, lens, 2, dtype)
+    q = randn((batch.T, 8, D), 64, dtype).to(cuda)
+    batch.k, batch.v, batch.table = batch.k.to(cuda), batch.v.to(cuda), batch.table.to(cuda)
+    exact, spread, score = paged.attn_paged(q, batch.k, batch.v, batch.table, batch.cu, lens, SCALE)
+    out = attend(batch, q, cuda)
+    finish()
+    total = batch.cu[-1]
+    close_to_attention(out[:total], exact[:total].cpu(), spread[:total].cpu(), score, max(lens), 6.0, dtype)
+    assert bool((out[total:].float() == 7.0).all())
+
+
+def test_a_batch_in_which_no_sequence_brings_anything(cuda, native_lib):
+    """A padded step whose ranges are all empty, by attention and by append: nothing is written."""
+    from neptune_mlir import runtime
+
+    batch = Batch([0, 0, 0], [5, 0, 200], 2, torch.bfloat16, pad=4)
+    q = randn((4, 8, D), 65, torch.bfloat16).to(cuda)
+    kv = randn((4, 2, D), 66, torch.bfloat16).to(cuda)
+    out = attend(batch, q, cuda)
+    kp, vp, q_out = batch.k.to(cuda), batch.v.to(cuda), torch.full_like(q, 7.0)
+    runtime.rope_append(q, kv, kv, kp, vp, *batch.device_args(cuda), torch.ones(64, device=cuda), q_out, rot_dim=D,
+                        interleaved=False, eps=1e-6, **batch.facts(8))
+    finish()
+    assert bool((out == 7.0).all()) and bool((q_out == 7.0).all())
+    assert torch.equal(kp.cpu().view(torch.int16), batch.k.view(torch.int16))
+    assert torch.equal(vp.cpu().view(torch.int16), batch.v.view(torch.int16))
+
+
+def test_rows_in_front_of_the_first_sequence_are_left_alone(cuda, native_lib):
+    """cu_seqlens that begins behind row 0, by attention and by append."""
+    from neptune_mlir import runtime
+
+    front = 5
+    batch = Batch([33, 1], [90, 300], 2, torch.bfloat16)
+    q = randn((batch.T, 8, D), 67, torch.bfloat16)
+    kv = randn((front + batch.T, 2, D), 68, torch.bfloat16).to(cuda)
+    wide = torch.cat([torch.full((front, 8, D), float("nan"), dtype=q.dtype), q]).to(cuda)
+    table, cu, lens = batch.device_args(cuda)
+    out, q_out = torch.full_like(wide, 7.0), torch.full_like(wide, 7.0)
+    facts = {**batch.facts(8), "T": front + batch.T}
+    work = torch.empty(runtime.attn_paged_workspace_bytes(), dtype=torch.uint8, device=cuda)
+    runtime.attn_paged(wide, batch.k.to(cuda), batch.v.to(cuda), table, cu + front, lens, work, out,
+                       scale_log2=SCALE * math.log2(math.e), **facts)
+    freq = 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float32) / D)
+    kp, vp = batch.k.to(cuda), batch.v.to(cuda)
+    runtime.rope_append(wide, kv, kv, kp, vp, table, cu + front, lens, freq.to(cuda), q_out, rot_dim=D, interleaved=False,
+                        eps=1e-6, **facts)
+    finish()
+    assert bool((out[:front] == 7.0).all()) and bool((q_out[:front] == 7.0).all())
+    exact, spread, score = paged.attn_paged(q, batch.k, batch.v, batch.table, batch.cu, batch.lens, SCALE)
+    total = batch.cu[-1]
+    close_to_attention(out[front:front + total], exact[:total], spread[:total], score, 300, 6.0, torch.bfloat16)
+    where = paged.positions_of(batch.cu, batch.lens)
+    exact, size = paged.norm_rope(q[:total], None, torch.tensor([p for _, _, p in where]), freq, 1e-6, False)
+    close_to_rotation(q_out[front:front + total], exact, size, torch.bfloat16)
+    for t, b, p in where:
+        page, row = cache_row(batch, b, p)
+        assert torch.equal(vp[page, :, row], kv[front + t])
+
+
+def test_append_without_queries_through_the_custom_op(cuda, native_lib):
+    """q and q_out absent: keys and values alone, the same bits as beside queries."""
+    from neptune_mlir import torch_ops  # noqa: F401
+
+    batch = Batch([5, 70], [69, 70], 2, torch.bfloat16, pad=0)
+    q, k, v = (randn((batch.T, h, D), 69 + i, torch.bfloat16).to(cuda) for i, h in enumerate((4, 2, 2)))
+    freq = torch.linspace(0.1, 1.0, 64).to(cuda)
+    got = []
+    for queries in (q, None):
+        kp, vp = batch.k.to(cuda), batch.v.to(cuda)
+        q_out = None if queries is None else torch.empty_like(q)
+        torch.ops.nb200.rope_append(queries, k, v, kp, vp, *batch.device_args(cuda), freq, q_out, None, None, 1e-6, False)
+        got.append((kp.view(torch.int16), vp.view(torch.int16)))
+    finish()
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+    assert not torch.equal(got[0][0].cpu(), batch.k.view(torch.int16))
+
+
+def test_two_threads_attend_at_the_same_time(cuda, native_lib):
+    """A stream, a workspace and a batch each: neither waits for the other, neither reads the other's parts."""
+    import threading
+
+    from neptune_mlir import runtime
+
+    jobs = []
+    for seed, (new, lens) in enumerate((([3, 40], [5000, 300]), ([200], [2500]))):
+        batch = Batch(new, lens, 2, torch.bfloat16, seed=seed)
+        q = randn((batch.T, 8, D), 80 + seed, torch.bfloat16)
+        want = attend(batch, q.to(cuda), cuda)
+        on = (q.to(cuda), batch.k.to(cuda), batch.v.to(cuda), *batch.device_args(cuda))
+        outs = [torch.full((batch.T, 8, D), 7.0, dtype=torch.bfloat16, device=cuda) for _ in range(20)]
+        jobs.append((batch, on, torch.empty(runtime.attn_paged_workspace_bytes(), dtype=torch.uint8, device=cuda), outs, want))
+    torch.cuda.synchronize()
+    together, failed = threading.Barrier(2), []
+
+    def work(batch, on, scratch, outs, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(device=cuda)):
+                together.wait()
+                for out in outs:
+                    runtime.attn_paged(*on, scratch, out, scale_log2=SCALE * math.log2(math.e), **batch.facts(8))
+                torch.cuda.current_stream().synchronize()
+        except Exception as exc:
+            failed.append(exc)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    finish()
+    assert not failed
+    for _, _, _, outs, want in jobs:
+        for out in outs:
+            assert torch.equal(out, want)
