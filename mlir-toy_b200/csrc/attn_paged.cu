@@ -33,9 +33,10 @@
 // What bounds it.  A block takes 0.9 us where its products need 0.53: three blocks are in flight and the chain from PV(g-3)
 // over S(g) and its softmax to PV(g) is 2.6 us long.  A change of tiles costs about 2 us more.  Under sustained load the
 // power limit takes the clock from 1.9 to 1.3 - 1.5 GHz and both grow with it.  Measured, 32 / 8 heads, bf16:
-//   4096 tokens, nothing cached     141 us alone (975 TFLOP/s), 160 sustained; tensor pipe 48 % busy
-//   2048 tokens over 30000 rows     850 us alone (1250 TFLOP/s), 955 sustained
-//   32 sequences of up to 7 tokens, 40 / 8 heads, up to 16001 rows: 166 us, 1.04 GB read once at 6.3 TB/s; 176 sustained
+//   4096 tokens, nothing cached     141 us alone (975 TFLOP/s), 160 - 167 sustained; tensor pipe 48 % busy
+//   2048 tokens over 30000 rows     850 us alone (1225 TFLOP/s), 955 - 982 sustained
+//   32 sequences of up to 7 tokens, 40 / 8 heads, up to 16001 rows: 166 us, 1.04 GB read once at 6.3 TB/s; 171 - 182 sustained
+//   32 single tokens over 8000 rows each: 174 us sustained, 1.05 GB at 6.0 TB/s
 //
 // P is rounded to the storage type because the second product takes both operands in one 16-bit type; the row sum adds
 // the unrounded values.  The running maximum passes between the warpgroups through shared memory, O is rescaled only when
@@ -83,7 +84,11 @@ constexpr int kMaxCtas = 160;                   // CTAs that the workspace has r
 // single sequence whose K and V do not, and whose tiles are about equally long, is dealt out in waves first: every CTA
 // takes the same number of whole tiles, in order, so that neighbours read the same blocks at the same time, and only what
 // is left is cut.  2048 tokens over 30000 cached rows (131 MB): 0.15 GB of DRAM reads and 971 us under sustained load, 2.46 GB
-// and 1117 us without.
+// and 1117 us without.  "About equally long" (the shortest tile within an eighth of the longest) is on the safe side: a wave
+// lasts as long as its longest tile.  Sustained, as it is / in waves whatever the tiles' lengths / never in waves:
+//   8192 tokens over 30000 rows   5.08 / 4.39 / 4.98 ms        16384 over 8192    4.23 / 4.19 / 4.22
+//   20000, nothing cached         3.16 / 3.20 / 3.15           32768, nothing     9.11 / 8.49 / 9.05
+// So the bound gives something away at long caches.  Batches of more than one sequence have not been tried.
 constexpr long long kWaveBytes = 1ll << 26;     // half of the L2
 constexpr int kTileUnits = 2;                   // what changing tiles costs (2 us), in blocks, on the line that is cut
 

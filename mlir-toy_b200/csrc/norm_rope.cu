@@ -15,10 +15,11 @@
 // read from shared memory once for all the rows of the token.  No barrier wider than a warp; four rows' loads are in
 // flight at a time, the first four while the token's sequence, page and angles are looked up.
 //
-// What bounds it is HBM: 8 x 4096 tokens of 32 / 32 heads with norms in 185 us (5.8 TB/s, where a plain copy of the same
-// bytes takes 168), an append of 2 x 8192 tokens of 32 / 8 heads in 74 us (5.4 TB/s; builds that skipped the look-up of the
-// page, and the angles, took 2 and 1 us less).  Small calls are bound by the launch: 2.5 to 3.4 us on the GPU, 3.3 to 5 us
-// of host time.
+// What bounds it is HBM: 8 x 4096 tokens of 32 / 32 heads with norms in 185 us alone from idle clocks (5.8 TB/s, where a
+// plain copy of the same bytes takes 168), 192 to 199 one call after the other (5.4 TB/s); in fp32 335 us (6.4 TB/s).  An
+// append of 2 x 8192 tokens of 32 / 8 heads takes 74 us alone (5.4 TB/s), 76 one after the other (5.3); builds that skipped the
+// look-up of the page, and the angles, took 2 and 1 us less.  Small calls are bound by the launch: 2.5 to 3.4 us on the
+// GPU, 3.3 to 5 us of host time.
 #include "nb200_common.cuh"
 
 namespace nb200 {
