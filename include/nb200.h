@@ -313,7 +313,7 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  *   scale_log2 : log2(e) * softmax scale
  * At most 128 query heads to a kv head; T below 2^30, max_pages * page_size up to 2^30.  Two kernels: the second joins the
  * tiles that were worked on by more than one CTA, in an order that lengths alone decide, so that equal calls give equal
- * bits.  out shares no element with the other tensors.
+ * bits.  out shares no element with the other tensors (it may not be q).
  * A row that sees nothing (its position is negative) is 0, one whose visible scores are all -infinity is NaN, as its
  * softmax is; rows that belong to no sequence are not touched.  Cache rows
  * at and beyond a sequence's length are not used, whatever they hold; an infinite value makes that column of the

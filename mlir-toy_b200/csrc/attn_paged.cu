@@ -1156,6 +1156,7 @@ extern "C" int nb200_attn_paged(const void *q, const void *k_pages, const void *
                   "%s: the strides of q and out must be multiples of 16 bytes, at least a row", who);
   }
   NB200_REQUIRE(rows_apart(kD, {T, Hq}, {s[2], s[3]}), NB200_ERR_BAD_ARG, "%s: the rows of out must lie apart", who);
+  NB200_REQUIRE(q != out, NB200_ERR_BAD_ARG, "%s: out must not be q", who);   // a tile that is cut is read by several CTAs
   Args a{};
   a.block_table = block_table, a.cu_seqlens = cu_seqlens, a.seq_lens = seq_lens;
   a.out = static_cast<uint4 *>(out), a.out_t = static_cast<unsigned>(s[2] / 8), a.out_h = static_cast<unsigned>(s[3] / 8);

@@ -195,3 +195,11 @@ def test_the_batch_or_token_stride_of_an_extent_of_one_is_not_looked_at(native_l
         rc = lib.nb200_rope_append(p, p, p, p, p + 8, p, p, p, p, p, None, None, longs(*strides * 4), T, 1, H, H, 8, 4, 64, 128,
                                    128, 0, 1e-6, 1, None, None)
         assert rc == -1 and b"page pools" in lib.nb200_last_error(), (strides, lib.nb200_last_error())
+
+
+def test_attention_in_place_is_refused(native_lib, ptr):
+    """Several CTAs read a tile's queries after the first has written its part of the output."""
+    lib, p = native.load(str(native_lib)), ptr[0]
+    for strides in (longs(512, 128, 512, 128), longs(512, 128, 1024, 256)):
+        rc = lib.nb200_attn_paged(p, p, p, p, p, p, p, p, strides, 2, 1, 4, 2, 8, 4, 64, 128, 1, 0.1, None, None)
+        assert rc == -1 and b"out must not be q" in lib.nb200_last_error()
