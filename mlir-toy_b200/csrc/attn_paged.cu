@@ -147,6 +147,7 @@ struct Shared {
   int taint_any[2];                  // tile number + 1
   uint32_t tmem_base;
   int skip;
+  int error[3];                      // code (0: none), detail, thread
   int k_issued;                      // K blocks asked for: whoever waits for a whole tile sees that it goes on
   float mslot[2][kBM];               // running maximum decided by block g, slot g & 1
   float2 lm[2][2][kBM];              // of tile n in [n & 1], per warpgroup: (maximum last used, partial row sum)
@@ -156,8 +157,9 @@ constexpr int kOffStage = 6 * kTileBytes, kOffShared = kOffStage + 4 * kStage;
 constexpr int kSmemBytes = kOffShared + 1024 + static_cast<int>(sizeof(Shared));
 static_assert(kSmemBytes <= 232448, "shared memory of one CTA");
 
-__device__ __forceinline__ void report(int *status, int code, int detail) {
-  status_record(status, code, static_cast<int>(blockIdx.x), detail, static_cast<int>(threadIdx.x));
+// Notes an expired wait; the CTA records one of its notes in the status words at its end.
+__device__ __forceinline__ void report(Shared *sh, int code, int detail) {
+  if (sh->error[0] == 0) sh->error[0] = code, sh->error[1] = detail, sh->error[2] = static_cast<int>(threadIdx.x);
 }
 
 // Waits for a phase with a limit on the turns: about 2 s if every turn suspends the thread for its microsecond, at least
@@ -264,6 +266,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     sh->waves = 0;
     sh->taint_any[0] = sh->taint_any[1] = 0;
     sh->k_issued = 0;
+    sh->error[0] = 0;
   }
   if (warp == 13) {
     // one barrier per lane and turn
@@ -479,7 +482,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (page >= pages) return outside;
         const int e = table[page];
         if (e >= 0 && e < a.num_pages) return e * a.Hkv + kvh;
-        if (is_k) report(a.status, kStatusBadPage, e);
+        if (is_k) status_record(a.status, kStatusBadPage, static_cast<int>(blockIdx.x), e, static_cast<int>(threadIdx.x));
         return outside;
       };
       bool ok = true;
@@ -534,7 +537,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         if (!ok) break;
       }
       if (!ok && lane == 0) {
-        report(a.status, kErrProducer, 2 * g + (is_k ? 0 : 1));
+        report(sh, kErrProducer, 2 * g + (is_k ? 0 : 1));
         // Unwinding: let the copies already in flight land before the CTA's shared memory goes away.
         for (int spin = 0; spin < 100000; ++spin) {
           bool done = true;
@@ -601,7 +604,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           }
           if (ok) umma_commit(b_q_empty + 8 * (n & 1));
         }
-        if (!ok) report(a.status, kErrMma, 2 * g);
+        if (!ok) report(sh, kErrMma, 2 * g);
       }
       __syncwarp();
     } else {
@@ -652,7 +655,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
             if (j + 1 == nblk) umma_commit(b_o_full + 8 * (n & 3));
           }
         }
-        if (!ok) report(a.status, kErrMma, 2 * g + 1);
+        if (!ok) report(sh, kErrMma, 2 * g + 1);
       }
       __syncwarp();
     }
@@ -843,7 +846,7 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
         notes ^= 1;
       }
     }
-    if (!ok && lane == 0) report(a.status, kErrEpilogue, g0);
+    if (!ok && lane == 0) report(sh, kErrEpilogue, g0);
   } else {
     // ================================ softmax: warpgroup w takes the blocks g with g & 1 == w ================
     asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
@@ -995,12 +998,14 @@ attn_paged_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       tc_fence_before();
       mbar_arrive(b_p_full + 8 * sb);
     }
-    if (!ok && lane == 0) report(a.status, kErrSoftmax, g0);
+    if (!ok && lane == 0) report(sh, kErrSoftmax, g0);
   }
 
   // ================================ tear-down =====================================
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && sh->error[0] != 0)
+    status_record(a.status, sh->error[0], static_cast<int>(blockIdx.x), sh->error[1], sh->error[2]);
   if (warp == 15) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);

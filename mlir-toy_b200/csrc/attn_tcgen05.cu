@@ -73,14 +73,16 @@ struct Shared {
   uint32_t tmem_base;
   int abort_flag;
   int skip;
-  int pad;
+  int error[3];             // code (0: none), detail, thread
   float mslot[2][128];      // running maximum decided by block g, slot g & 1
   float lm[2][128][2];      // per warpgroup: (maximum last used, partial row sum) of the finished tile
 };
 constexpr int kSmemBytes = 6 * kTileBytes + 1024 + static_cast<int>(sizeof(Shared));
 
-__device__ __forceinline__ void report(int *status, int code, int detail) {
-  status_record(status, code, static_cast<int>(blockIdx.x), detail, static_cast<int>(threadIdx.x));
+// Notes an expired wait; the CTA records one of its notes in the status words at its end.  (Recorded at each of the 22
+// places, the code for it took 13 % of the time: 1.30 ms for 8 x 32 heads of 4096 rows, 1.11 like this.)
+__device__ __forceinline__ void report(Shared *sh, int code, int detail) {
+  if (sh->error[0] == 0) sh->error[0] = code, sh->error[1] = detail, sh->error[2] = static_cast<int>(threadIdx.x);
 }
 
 // Polling wait (mbarrier.test_wait never suspends the thread): the waiter continues a few cycles after the phase
@@ -155,6 +157,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 
   if (threadIdx.x == 0) {
     sh->abort_flag = 0;
+    sh->error[0] = 0;
     sh->skip = (status != nullptr && status_stops(*reinterpret_cast<volatile int *>(status))) ? 1 : 0;
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&sh->q_full[b]), 1);
@@ -234,13 +237,13 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             mbar_arrive(b_sched + 8 * (n % kSched));
           } else {
             i = tile_at(n);
-            if (i < 0) { report(status, kErrProducer, -1000 - n); ok = false; break; }
+            if (i < 0) { report(sh, kErrProducer, -1000 - n); ok = false; break; }
           }
           if (i >= prob.total) break;
           const Tile t = tile_of(prob, i);
           if (is_k) {
             ok = mbar_wait(b_q_empty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag);
-            if (!ok) { report(status, kErrProducer, -1 - n); break; }
+            if (!ok) { report(sh, kErrProducer, -1 - n); break; }
             mbar_arrive_expect_tx(b_q_full + 8 * (n & 1), kTileBytes);
             tma_load_3d(sQ + (n & 1) * kTileBytes, &tm_q, 0, t.qt * kBM, t.bh, b_q_full + 8 * (n & 1));
             tma_load_3d(sQ + (n & 1) * kTileBytes + kBox, &tm_q, 64, t.qt * kBM, t.bh, b_q_full + 8 * (n & 1));
@@ -249,7 +252,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           for (int j = 0; j < t.nblk && ok; ++j, ++g) {
             const int b = g & 1;
             ok = mbar_wait(b_empty + 8 * b, ((g >> 1) & 1) ^ 1, abort_flag);
-            if (!ok) { report(status, kErrProducer, 2 * g + (is_k ? 0 : 1)); break; }
+            if (!ok) { report(sh, kErrProducer, 2 * g + (is_k ? 0 : 1)); break; }
             mbar_arrive_expect_tx(b_full + 8 * b, kTileBytes);
             tma_load_3d(s_dst + b * kTileBytes, tm, 0, j * kBN, t.bh, b_full + 8 * b);
             tma_load_3d(s_dst + b * kTileBytes + kBox, tm, 64, j * kBN, t.bh, b_full + 8 * b);
@@ -294,19 +297,19 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         int g = 0;
         for (int n = 0; ok; ++n) {
           const int i = tile_at(n);
-          if (i < 0) { report(status, kErrMma, -1000 - n); break; }
+          if (i < 0) { report(sh, kErrMma, -1000 - n); break; }
           if (i >= prob.total) break;
           const int nblk = tile_of(prob, i).nblk;
           ok = mbar_wait(b_q_full + 8 * (n & 1), (n >> 1) & 1, abort_flag);
-          if (!ok) { report(status, kErrMma, -1 - n); break; }
+          if (!ok) { report(sh, kErrMma, -1 - n); break; }
           const uint32_t q_step = (n & 1) * kStageStep;
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = mbar_wait(b_k_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
-            if (!ok) { report(status, kErrMma, 4 * g); break; }
+            if (!ok) { report(sh, kErrMma, 4 * g); break; }
             if (g >= kSBufs) {
               ok = mbar_wait_poll(b_pv_done + 8 * sb, ((g - kSBufs) / kSBufs) & 1, abort_flag);
-              if (!ok) { report(status, kErrMma, 4 * g + 1); break; }
+              if (!ok) { report(sh, kErrMma, 4 * g + 1); break; }
             }
             tc_fence_after();
             const uint32_t d_tmem = tmem + sb * 128, k_step = (g & 1) * kStageStep;
@@ -334,19 +337,19 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         int g = 0;
         for (int n = 0; ok; ++n) {
           const int i = tile_at(n);
-          if (i < 0) { report(status, kErrMma, -1000 - n); break; }
+          if (i < 0) { report(sh, kErrMma, -1000 - n); break; }
           if (i >= prob.total) break;
           const int nblk = tile_of(prob, i).nblk;
           for (int j = 0; j < nblk && ok; ++j, ++g) {
             const int sb = g % kSBufs;
             ok = mbar_wait(b_v_full + 8 * (g & 1), (g >> 1) & 1, abort_flag);
-            if (!ok) { report(status, kErrMma, 4 * g + 2); break; }
+            if (!ok) { report(sh, kErrMma, 4 * g + 2); break; }
             if (j == 0 && n > 0) {   // the epilogue of the previous tile has read O
               ok = mbar_wait(b_o_free, (n - 1) & 1, abort_flag);
-              if (!ok) { report(status, kErrMma, 4 * g + 3); break; }
+              if (!ok) { report(sh, kErrMma, 4 * g + 3); break; }
             }
             ok = mbar_wait_poll(b_p_full + 8 * sb, (g / kSBufs) & 1, abort_flag);
-            if (!ok) { report(status, kErrMma, 4 * g + 3); break; }
+            if (!ok) { report(sh, kErrMma, 4 * g + 3); break; }
             tc_fence_after();
             const uint32_t p_tmem = tmem + sb * 128, v_step = (g & 1) * kStageStep;
 #pragma unroll
@@ -368,18 +371,18 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     bool ok = true;
     for (int n = 0;; ++n) {
       const int i = __shfl_sync(0xffffffffu, tile_at(n), 0);
-      if (i < 0) { report(status, kErrEpilogue, -1000 - n); break; }
+      if (i < 0) { report(sh, kErrEpilogue, -1000 - n); break; }
       if (i >= prob.total) break;
       const Tile t = tile_of(prob, i);
       ok = __all_sync(0xffffffffu, mbar_wait(b_lm_ready, n & 1, abort_flag));
-      if (!ok) { report(status, kErrEpilogue, 2 * n); break; }
+      if (!ok) { report(sh, kErrEpilogue, 2 * n); break; }
       const float m0 = sh->lm[0][r][0], l0 = sh->lm[0][r][1], m1 = sh->lm[1][r][0], l1 = sh->lm[1][r][1];
       mbar_arrive(b_lm_free);
       const float mf = fmaxf(m0, m1);   // the running maximum never decreases: the later one is the larger
       const float l = (l0 > 0.f ? l0 * ex2(m0 - mf) : 0.f) + (l1 > 0.f ? l1 * ex2(m1 - mf) : 0.f);
       const float inv = 1.f / l;
       ok = __all_sync(0xffffffffu, mbar_wait(b_o_full, n & 1, abort_flag));
-      if (!ok) { report(status, kErrEpilogue, 2 * n + 1); break; }
+      if (!ok) { report(sh, kErrEpilogue, 2 * n + 1); break; }
       tc_fence_after();
       const int q_row = t.qt * kBM + r;
       uint16_t *dst = out + (static_cast<size_t>(t.bh) * prob.Sq + q_row) * kD;
@@ -415,7 +418,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     int n = 0, g0 = 0;
     int i = __shfl_sync(0xffffffffu, tile_at(0), 0);
     bool ok = i >= 0;
-    if (!ok) report(status, kErrSoftmax, -1000);
+    if (!ok) report(sh, kErrSoftmax, -1000);
     Tile t = (ok && i < prob.total) ? tile_of(prob, i) : Tile{0, 0, 0};
     float m_mine = -INFINITY, l = 0.f;
     for (int g = w; ok; g += 2) {
@@ -423,7 +426,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       while (i < prob.total && g >= g0 + t.nblk) {
         if (n > 0) {   // the epilogue has read the previous tile's values
           ok = __all_sync(0xffffffffu, mbar_wait(b_lm_free, (n - 1) & 1, abort_flag));
-          if (!ok) { report(status, kErrSoftmax, -1 - n); break; }
+          if (!ok) { report(sh, kErrSoftmax, -1 - n); break; }
         }
         sh->lm[w][r][0] = m_mine;
         sh->lm[w][r][1] = l;
@@ -433,7 +436,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         g0 += t.nblk;
         ++n;
         i = __shfl_sync(0xffffffffu, tile_at(n), 0);
-        if (i < 0) { report(status, kErrSoftmax, -1000 - n); ok = false; break; }
+        if (i < 0) { report(sh, kErrSoftmax, -1000 - n); ok = false; break; }
         if (i < prob.total) t = tile_of(prob, i);
       }
       if (!ok || i >= prob.total) break;
@@ -441,13 +444,13 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const int sb = g % kSBufs;
       const uint32_t tS = tmem + sb * 128 + lane_addr;
       ok = __all_sync(0xffffffffu, mbar_wait(b_s_full + 8 * sb, (g / kSBufs) & 1, abort_flag));
-      if (!ok) { report(status, kErrSoftmax, g); break; }
+      if (!ok) { report(sh, kErrSoftmax, g); break; }
       tc_fence_after();
       float m_prev = 0.f;
       if (g > 0) {
         // block g-1 has decided on its maximum (and, before that, has read the slot this block will overwrite)
         ok = __all_sync(0xffffffffu, mbar_wait(b_m_ready + 8 * ((g - 1) & 1), ((g - 1) >> 1) & 1, abort_flag));
-        if (!ok) { report(status, kErrSoftmax, 1000 + g); break; }
+        if (!ok) { report(sh, kErrSoftmax, 1000 + g); break; }
         if (j > 0) m_prev = sh->mslot[(g - 1) & 1][r];
       }
       uint32_t v[kBN];
@@ -489,7 +492,7 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       if (__any_sync(0xffffffffu, need)) {
         // O must hold every product up to block g-1 and none may be in flight
         ok = __all_sync(0xffffffffu, mbar_wait(b_pv_done + 8 * ((g - 1) % kSBufs), ((g - 1) / kSBufs) & 1, abort_flag));
-        if (!ok) { report(status, kErrSoftmax, 2000 + g); break; }
+        if (!ok) { report(sh, kErrSoftmax, 2000 + g); break; }
         tc_fence_after();
         const float f = need ? ex2(m_prev - m_blk) : 1.f;
 #pragma unroll 1
@@ -537,6 +540,8 @@ attn_fwd_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   // ================================ tear-down =====================================
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && sh->error[0] != 0)
+    status_record(status, sh->error[0], static_cast<int>(blockIdx.x), sh->error[1], sh->error[2]);
   if (warp == 15) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
