@@ -264,8 +264,8 @@ int nb200_decode_fwd_static(const void *q, const void *k, const void *v, void *o
  *   strides   : HOST array of 13: the batch, token and head stride (in elements) of q, k, q_out and k_out in this order,
  *               then the batch stride of positions (0: one row for all).  Rows are contiguous; strides and base
  *               addresses are multiples of 16 bytes, but for the batch or token stride of an extent of 1, which is not
- *               used.  So q and k may be views into a packed projection and q_out,
- *               k_out [B, H, S, D] tensors as nb200_attn_fwd reads them.
+ *               used.  So q and k may be views into a packed projection and q_out, k_out [B, H, S, D] tensors as
+ *               nb200_attn_fwd reads them.
  * An output may be its own input (same address and strides); otherwise outputs share no element with inputs.  An output's
  * rows lie apart, and its dimensions nest: taken by size, a stride that does not cover what the smaller ones reach is refused,
  * unless its extent is 1.
@@ -315,11 +315,10 @@ int nb200_rope_append(const void *q, const void *k, const void *v, void *q_out, 
  * tiles that were worked on by more than one CTA, in an order that lengths alone decide, so that equal calls give equal
  * bits.  out shares no element with the other tensors (it may not be q).
  * A row that sees nothing (its position is negative) is 0, one whose visible scores are all -infinity is NaN, as its
- * softmax is; rows that belong to no sequence are not touched.  Cache rows
- * at and beyond a sequence's length are not used, whatever they hold; an infinite value makes that column of the
- * rows that see it infinite (NaN beside one of the other sign, and it may where its weight rounds to 0), a NaN makes it
- * NaN; neither reaches another row.  A table entry outside [0, num_pages) is never
- * dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and
+ * softmax is; rows that belong to no sequence are not touched.  Cache rows at and beyond a sequence's length are not used,
+ * whatever they hold.  An infinite value makes that column of the rows that see it infinite (NaN beside one of the other
+ * sign, and it may where its weight rounds to 0), a NaN makes it NaN; neither reaches another row.  A table entry outside
+ * [0, num_pages) is never dereferenced: rows that would read it become NaN (rows of the same sequence that are computed with them may too) and
  * `status` records code 22.
  */
 size_t nb200_attn_paged_workspace_bytes(void);

@@ -78,8 +78,8 @@ def status_buffer(dev: torch.device) -> torch.Tensor:
     """Per-device int32[4] that kernels with bounded device-side waits report into.
 
     Made once per device, whichever threads ask first: the native binding keeps the address (_first_status_buffer), so
-    there is one tensor and it stays.  The stream that clears it is waited for, because every stream of the device uses it from then
-    on.  A graph capture cannot wait: words made inside one are that call's alone, cleared by each replay.
+    there is one tensor and it stays.  The stream that clears it is waited for, because every stream of the device uses
+    it from then on.  A graph capture cannot wait: words made inside one are that call's alone, cleared by each replay.
     """
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     buf = _status_buffers.get(idx)
